@@ -15,9 +15,12 @@
  *     device" (the reference's skip code, include/kernelh/runtime/
  *     runtime_error.hpp:15-20), 2 means a usage error (unknown kernel, bad
  *     shape, wrong buffer count), 1001 means a device-side bounded wait ran
- *     out, any other value is the driver's error code.
+ *     out, 1002 that a kernel read an index from device memory that lies
+ *     outside its table (kh_synchronize; the access was skipped), any other
+ *     value is the driver's error code.
  *   - kh_last_error() returns the message of the calling thread's last failure.
- *   - Tensors are fp32, row-major, contiguous. Device-pointer calls enqueue on
+ *   - Tensors are fp32, row-major, contiguous, unless an entry says otherwise
+ *     (those that take kh_head_rows or kh_paged_rows). Device-pointer calls enqueue on
  *     `stream` (a CUstream / cudaStream_t, NULL = default stream) and return
  *     without waiting. There is no CPU path: without a B200 the compute calls
  *     fail with 77 or the driver's error.
@@ -258,6 +261,73 @@ int kh_arm_arrival_flags(kh_context *ctx, void *const *flag_arrays, int world, u
  * kh_synchronize waits for it and reports a wait that ran out (1001) like any other. */
 int kh_arm_arrival_flags_overlapped(kh_context *ctx, void *const *flag_arrays, int world, uint64_t epoch);
 int kh_join_arrivals(kh_context *ctx, void *stream);
+
+/* ---- attention with a cache: norms, rotation, paged cache -------------------
+ * No counterparts in the reference, whose attention takes whole fp32 tensors of
+ * one length and 64-value heads (lib/dsl/kernels/attention.cpp:109-120) and whose
+ * norm is the layernorm over whole rows. These are the operators between a
+ * projection's output and its attention, in fp32, bf16 or fp16 (arithmetic in
+ * fp32, one rounding at the end), on any stream, with no scratch of the context:
+ * where one is needed the caller passes it, so calls on several streams, and
+ * graphs that hold such calls, do not share anything unless the caller makes them.
+ */
+enum { KH_F32 = 0, KH_BF16 = 1, KH_F16 = 2 };
+/* tokens x heads rows of head_dim contiguous values: row (t, h) starts
+ * t * token_stride + h * head_stride elements after `data`. The stride of a
+ * dimension of size 1 is not read. Parts of one buffer (queries, keys and values
+ * of a joint projection), or [heads, tokens, head_dim] order, need no copy. */
+typedef struct {
+  void *data;
+  int64_t token_stride, head_stride;
+} kh_head_rows;
+/* A paged cache: slot s of page p holds one row per head, `data` + p * page_stride
+ * + s * slot_stride + h * head_stride. */
+typedef struct {
+  void *data;
+  int64_t page_stride, slot_stride, head_stride;
+} kh_paged_rows;
+
+/* The RMS norm of every head of q and k with learned weights, and the rotation of
+ * positions, in one pass over both. For a row x: n = x * weight / sqrt(mean(x^2) +
+ * eps); then the first rotary_dim values are rotated by position * inv_freq[j],
+ * j < rotary_dim / 2, in the pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) when
+ * `interleaved`; the others stay. head_dim: even, at most 256; rotary_dim: even,
+ * 0 .. head_dim. Weights (head_dim fp32 values) may be NULL: ones. `positions`: one
+ * per token, any 64-bit value that keeps position * inv_freq below 2^52. Angles are
+ * formed in 64 bits. Outputs may be the inputs themselves (same address and
+ * strides); any other overlap is the caller's error. tokens = 0 is allowed. */
+typedef struct {
+  int32_t dtype; /* KH_F32, KH_BF16, KH_F16: of all rows */
+  int32_t q_heads, k_heads, head_dim, rotary_dim, interleaved;
+  float eps;
+  int64_t tokens;
+  kh_head_rows q, k;
+  const float *q_weight, *k_weight;
+  const float *inv_freq;
+  const int64_t *positions;
+} kh_qk_norm_rope_args;
+int kh_qk_norm_rope(kh_context *ctx, const kh_qk_norm_rope_args *args, kh_head_rows q_out, kh_head_rows k_out,
+                    void *stream);
+/* Its backward pass: args as in the forward call (q and k its inputs), dq_out and
+ * dk_out the gradients of its outputs; dq, dk those of q and k (they may be dq_out
+ * and dk_out, or q and k, themselves); dq_weight, dk_weight: head_dim fp32 sums over
+ * all tokens and heads, overwritten, either may be NULL. The sums are formed in a
+ * fixed order: the same call gives the same bits. `workspace`: device memory of
+ * kh_qk_norm_rope_backward_workspace(head_dim) bytes, 4-byte aligned, any contents. */
+int64_t kh_qk_norm_rope_backward_workspace(int32_t head_dim);
+int kh_qk_norm_rope_backward(kh_context *ctx, const kh_qk_norm_rope_args *args, kh_head_rows dq_out,
+                             kh_head_rows dk_out, kh_head_rows dq, kh_head_rows dk, float *dq_weight,
+                             float *dk_weight, void *workspace, int64_t workspace_bytes, void *stream);
+/* The serving form: the finished queries go to q_out, the finished keys and the
+ * values `v` (k_heads rows per token, copied) into a paged cache of num_pages pages
+ * of page_size slots. slots[t] = page * page_size + slot is where token t goes, -1:
+ * nowhere (padding of a captured batch). The slots of a call are distinct; of two
+ * tokens with one slot, which row is left there is not defined. A slot outside the
+ * cache stores nothing and is reported by kh_synchronize (1002). Rows of the cache
+ * that no slot names are not touched. */
+int kh_qk_norm_rope_append(kh_context *ctx, const kh_qk_norm_rope_args *args, kh_head_rows v,
+                           const int64_t *slots, kh_head_rows q_out, kh_paged_rows k_cache,
+                           kh_paged_rows v_cache, int64_t num_pages, int32_t page_size, void *stream);
 
 /* The SM clock the last gemm launch of this context really ran at: block 0 of the
  * kernel counts its SM's cycles against the GPU's nanosecond timer over its whole

@@ -20,6 +20,7 @@ LIB_PATH = os.path.join(_PKG, "libkernelh_b200.so")
 DRIVER_UNAVAILABLE = 77
 USAGE_ERROR = 2
 DEVICE_TIMEOUT = 1001
+BAD_DEVICE_INDEX = 1002
 
 KERNELS = ("attention", "fused_gelu", "gemm", "layernorm", "scan", "softmax", "vecadd")
 # the reference also registers the second kernel of its two-launch scan; here it launches nothing
@@ -57,6 +58,22 @@ class PlanInfo(C.Structure):
                 ("grid", C.c_uint32 * 3), ("block", C.c_uint32 * 3), ("dynamic_smem", C.c_int64),
                 ("param_count", C.c_int32), ("tmem_columns", C.c_int32), ("work", C.c_double),
                 ("work_is_flops", C.c_int32)]
+
+
+class HeadRows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class PagedRows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("page_stride", C.c_int64), ("slot_stride", C.c_int64),
+                ("head_stride", C.c_int64)]
+
+
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("q_heads", C.c_int32), ("k_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float), ("tokens", C.c_int64),
+                ("q", HeadRows), ("k", HeadRows), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p),
+                ("inv_freq", C.c_void_p), ("positions", C.c_void_p)]
 
 
 def _load() -> C.CDLL:
@@ -100,6 +117,12 @@ def _load() -> C.CDLL:
     L.kh_gemm_host_sharded_finish.argtypes = [vp, f32p]
     L.kh_attention.argtypes = [vp, f32p, f32p, f32p, f32p, i64, i64, i64, i64, vp]
     L.kh_attention_allgather.argtypes = [vp, f32p, f32p, f32p, C.POINTER(vp), vp, C.c_int, C.c_int, i64, i64, i64, vp]
+    rope = C.POINTER(QkNormRopeArgs)
+    L.kh_qk_norm_rope.argtypes = [vp, rope, HeadRows, HeadRows, vp]
+    L.kh_qk_norm_rope_backward_workspace.argtypes = [C.c_int32]
+    L.kh_qk_norm_rope_backward_workspace.restype = i64
+    L.kh_qk_norm_rope_backward.argtypes = [vp, rope, HeadRows, HeadRows, HeadRows, HeadRows, f32p, f32p, vp, i64, vp]
+    L.kh_qk_norm_rope_append.argtypes = [vp, rope, HeadRows, vp, HeadRows, PagedRows, PagedRows, i64, C.c_int32, vp]
     L.kh_malloc.argtypes = [vp, C.c_size_t, C.POINTER(vp)]
     L.kh_free.argtypes = [vp, vp]
     L.kh_memcpy_h2d.argtypes = [vp, vp, vp, C.c_size_t]
@@ -166,6 +189,25 @@ def _ptr(x) -> int | None:
     raise TypeError(f"cannot take the address of {type(x)!r}")
 
 
+# dtype codes of the entry points that take rows of more than one type, by the name torch gives the type
+_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+_dtype_codes: dict = {}  # the same by dtype object, filled as types are met (str() of a dtype is slow)
+
+
+def _refuse(message: str):
+    raise KernelhError(USAGE_ERROR, message)
+
+
+def _dtype_code(t, name: str) -> int:
+    code = _dtype_codes.get(t.dtype)
+    if code is None:
+        code = _DTYPES.get(str(t.dtype))
+        if code is None:
+            _refuse(f"'{name}' must be float32, bfloat16 or float16, got {t.dtype}")
+        _dtype_codes[t.dtype] = code
+    return code
+
+
 def shape_text(**shape: int) -> str:
     return ",".join(f"{k}={int(v)}" for k, v in shape.items())
 
@@ -178,6 +220,7 @@ class Context:
         h = C.c_void_p()
         _check(lib.kh_context_create(device_ordinal, C.byref(h)))
         self._h = h
+        self._ordinal = device_ordinal
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -341,6 +384,107 @@ class Context:
         _check(lib.kh_attention_allgather(self._h, _ptr(q), _ptr(k), _ptr(v), arr,
                                           C.c_void_p(int(o_multicast)) if o_multicast else None,
                                           len(o_replicas), rank, slices, seq, head_dim, stream))
+
+    # ---- norms, rotation and a paged cache -----------------------------------------
+    # These take torch tensors and read shapes, strides and types from them.
+    def _on_device(self, t, name: str, dtype: str | None = None, size: int | None = None) -> int:
+        """Address of a contiguous vector on this context's device, of `dtype` and `size` values."""
+        if not t.is_cuda or t.get_device() != self._ordinal:
+            _refuse(f"'{name}' must be on device {self._ordinal} of this context, got {t.device}")
+        if dtype is not None and str(t.dtype) != dtype:
+            _refuse(f"'{name}' must be {dtype}, got {t.dtype}")
+        if size is not None and t.numel() != size:
+            _refuse(f"'{name}' must have {size} values, got {t.numel()}")
+        if not t.is_contiguous():
+            _refuse(f"'{name}' must be contiguous")
+        return t.data_ptr()
+
+    def _rows(self, t, name: str, shape, code: int) -> HeadRows:
+        """A [tokens, heads, head_dim] tensor as rows: any strides but the last, which must be 1."""
+        if not t.is_cuda or t.get_device() != self._ordinal:
+            _refuse(f"'{name}' must be on device {self._ordinal} of this context, got {t.device}")
+        if t.shape != shape:
+            _refuse(f"'{name}' must have shape {tuple(shape)}, got {tuple(t.shape)}")
+        if _dtype_code(t, name) != code:
+            _refuse(f"'{name}' must have the type of 'q', got {t.dtype}")
+        s0, s1, s2 = t.stride()
+        if s2 != 1 and shape[2] != 1:
+            _refuse(f"'{name}': the values of a head must be contiguous (last stride {s2})")
+        return HeadRows(t.data_ptr(), s0, s1)
+
+    def _cache(self, t, name: str, shape, code: int) -> PagedRows:
+        """A [pages, page_size, heads, head_dim] tensor as a paged cache: any strides but the last."""
+        if not t.is_cuda or t.get_device() != self._ordinal:
+            _refuse(f"'{name}' must be on device {self._ordinal} of this context, got {t.device}")
+        if t.dim() != 4 or tuple(t.shape) != shape:
+            _refuse(f"'{name}' must have shape {shape}, got {tuple(t.shape)}")
+        if _dtype_code(t, name) != code:
+            _refuse(f"'{name}' must have the type of 'q', got {t.dtype}")
+        s0, s1, s2, s3 = t.stride()
+        if s3 != 1 and shape[3] != 1:
+            _refuse(f"'{name}': the values of a head must be contiguous (last stride {s3})")
+        return PagedRows(t.data_ptr(), s0, s1, s2)
+
+    def _qk_norm_rope_args(self, q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved) -> QkNormRopeArgs:
+        if q.dim() != 3 or k.dim() != 3:
+            _refuse("'q' and 'k' must be [tokens, heads, head_dim]")
+        code = _dtype_code(q, "q")
+        tokens, q_heads, head_dim = q.shape
+        k_heads = k.shape[1]
+        rotary = 2 * inv_freq.numel() if inv_freq is not None else 0
+        return QkNormRopeArgs(
+            code, q_heads, k_heads, head_dim, rotary, 1 if interleaved else 0, eps, tokens,
+            self._rows(q, "q", q.shape, code), self._rows(k, "k", (tokens, k_heads, head_dim), code),
+            None if q_weight is None else self._on_device(q_weight, "q_weight", "torch.float32", head_dim),
+            None if k_weight is None else self._on_device(k_weight, "k_weight", "torch.float32", head_dim),
+            None if inv_freq is None else self._on_device(inv_freq, "inv_freq", "torch.float32"),
+            self._on_device(positions, "positions", "torch.int64", tokens))
+
+    def qk_norm_rope(self, q, k, q_weight, k_weight, inv_freq, positions, q_out, k_out, eps=1e-6, interleaved=False,
+                     stream=None):
+        """RMS norm of every head of `q` [tokens, q_heads, head_dim] and `k` [tokens, k_heads, head_dim] (float32,
+        bfloat16 or float16, any token and head strides) with fp32 weights [head_dim] (None: ones), then the rotation
+        of the first 2 * len(inv_freq) values by positions * inv_freq: pairs (j, j + len(inv_freq)), or (2j, 2j + 1)
+        when `interleaved`. `inv_freq` fp32 (None: norms only), `positions` int64 [tokens]. `q_out`, `k_out` may be
+        `q`, `k` themselves."""
+        a = self._qk_norm_rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+        _check(lib.kh_qk_norm_rope(self._h, a, self._rows(q_out, "q_out", q.shape, a.dtype),
+                                   self._rows(k_out, "k_out", k.shape, a.dtype), stream))
+
+    def qk_norm_rope_backward_workspace(self, q, k) -> int:
+        """Bytes of device memory that `qk_norm_rope_backward` needs for such tensors."""
+        return int(lib.kh_qk_norm_rope_backward_workspace(q.shape[-1]))
+
+    def qk_norm_rope_backward(self, q, k, q_weight, k_weight, inv_freq, positions, dq_out, dk_out, dq, dk, dq_weight,
+                              dk_weight, workspace, eps=1e-6, interleaved=False, stream=None):
+        """Gradients of `qk_norm_rope` at the same arguments: from `dq_out`, `dk_out` (of its outputs) to `dq`, `dk`
+        (of q and k; they may be dq_out and dk_out themselves) and the fp32 sums `dq_weight`, `dk_weight` [head_dim]
+        (None: not wanted). Deterministic. `workspace`: any contiguous tensor of
+        `qk_norm_rope_backward_workspace(q, k)` bytes."""
+        a = self._qk_norm_rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+        d = a.head_dim
+        _check(lib.kh_qk_norm_rope_backward(
+            self._h, a, self._rows(dq_out, "dq_out", q.shape, a.dtype), self._rows(dk_out, "dk_out", k.shape, a.dtype),
+            self._rows(dq, "dq", q.shape, a.dtype), self._rows(dk, "dk", k.shape, a.dtype),
+            None if dq_weight is None else self._on_device(dq_weight, "dq_weight", "torch.float32", d),
+            None if dk_weight is None else self._on_device(dk_weight, "dk_weight", "torch.float32", d),
+            self._on_device(workspace, "workspace"), workspace.numel() * workspace.element_size(), stream))
+
+    def qk_norm_rope_append(self, q, k, v, q_weight, k_weight, inv_freq, positions, slots, q_out, k_cache, v_cache,
+                            eps=1e-6, interleaved=False, stream=None):
+        """`qk_norm_rope` that stores the finished keys, and the values `v`, into a paged cache: `k_cache`, `v_cache`
+        [pages, page_size, k_heads, head_dim] (any strides but the last). `slots` int64 [tokens]: page * page_size +
+        place of each token, -1 for a token that is not stored. A slot outside the cache is skipped and makes the next
+        `synchronize` raise (BAD_DEVICE_INDEX)."""
+        a = self._qk_norm_rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+        if k_cache.dim() != 4:
+            _refuse("'k_cache' must be [pages, page_size, k_heads, head_dim]")
+        pages, page_size = k_cache.shape[:2]
+        shape = (pages, page_size, a.k_heads, a.head_dim)
+        _check(lib.kh_qk_norm_rope_append(
+            self._h, a, self._rows(v, "v", k.shape, a.dtype), self._on_device(slots, "slots", "torch.int64", a.tokens),
+            self._rows(q_out, "q_out", q.shape, a.dtype), self._cache(k_cache, "k_cache", shape, a.dtype),
+            self._cache(v_cache, "v_cache", shape, a.dtype), pages, page_size, stream))
 
     # ---- raw device memory -------------------------------------------------------
     def malloc(self, nbytes: int) -> int:

@@ -352,6 +352,51 @@ int kh_attention_allgather(kh_context *ctx, const float *q, const float *k, cons
   });
 }
 
+namespace {
+int norm_rope(kh_context *ctx, const char *entry, const kh::NormRopeCall &call, void *stream) {
+  return guarded([&] {
+    if (auto r = kh::check_qk_norm_rope(entry, call); !r) return set_error(r.error());
+    if (int rc = need_ctx(ctx)) return rc;
+    auto r = kh::run_qk_norm_rope(*ctx->exec, call, stream);
+    return r ? 0 : set_error(r.error());
+  });
+}
+} // namespace
+
+int kh_qk_norm_rope(kh_context *ctx, const kh_qk_norm_rope_args *args, kh_head_rows q_out, kh_head_rows k_out,
+                    void *stream) {
+  if (args == nullptr) return set_error(2, "kh_qk_norm_rope: null arguments");
+  kh::NormRopeCall c{};
+  c.args = *args;
+  c.q_out = q_out, c.k_out = k_out;
+  return norm_rope(ctx, "kh_qk_norm_rope", c, stream);
+}
+int64_t kh_qk_norm_rope_backward_workspace(int32_t head_dim) { return kh::qk_norm_rope_backward_workspace(head_dim); }
+int kh_qk_norm_rope_backward(kh_context *ctx, const kh_qk_norm_rope_args *args, kh_head_rows dq_out,
+                             kh_head_rows dk_out, kh_head_rows dq, kh_head_rows dk, float *dq_weight,
+                             float *dk_weight, void *workspace, int64_t workspace_bytes, void *stream) {
+  if (args == nullptr) return set_error(2, "kh_qk_norm_rope_backward: null arguments");
+  kh::NormRopeCall c{};
+  c.kind = kh::NormRopeCall::Backward;
+  c.args = *args;
+  c.q_out = dq, c.k_out = dk, c.dq_out = dq_out, c.dk_out = dk_out;
+  c.dq_weight = dq_weight, c.dk_weight = dk_weight;
+  c.workspace = workspace, c.workspace_bytes = workspace_bytes;
+  return norm_rope(ctx, "kh_qk_norm_rope_backward", c, stream);
+}
+int kh_qk_norm_rope_append(kh_context *ctx, const kh_qk_norm_rope_args *args, kh_head_rows v,
+                           const int64_t *slots, kh_head_rows q_out, kh_paged_rows k_cache,
+                           kh_paged_rows v_cache, int64_t num_pages, int32_t page_size, void *stream) {
+  if (args == nullptr) return set_error(2, "kh_qk_norm_rope_append: null arguments");
+  kh::NormRopeCall c{};
+  c.kind = kh::NormRopeCall::Append;
+  c.args = *args;
+  c.v = v, c.slots = slots, c.q_out = q_out;
+  c.k_cache = k_cache, c.v_cache = v_cache;
+  c.num_pages = num_pages, c.page_size = page_size;
+  return norm_rope(ctx, "kh_qk_norm_rope_append", c, stream);
+}
+
 int kh_malloc(kh_context *ctx, size_t bytes, void **out) {
   if (int rc = need_ctx(ctx)) return rc;
   if (out == nullptr) return set_error(2, "kh_malloc: null out pointer");

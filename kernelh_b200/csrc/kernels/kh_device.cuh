@@ -28,7 +28,9 @@ namespace khd {
 // pipelines): status[0] == 0 means clean; a wait that runs out of its
 // iteration budget stores a non-zero code (first writer wins) and the kernel
 // stops issuing work and returns. The host reads the word after the stream
-// sync and maps it to an error. No trap, no device assert.
+// sync and maps it to an error. No trap, no device assert. An index that a
+// kernel reads from device memory and finds out of range is reported the same
+// way, after the access has been skipped.
 enum : uint32_t {
   kStatusOk = 0,
   kStatusScanLookbackTimeout = 1,
@@ -37,6 +39,9 @@ enum : uint32_t {
   kStatusEpilogueWaitTimeout = 4,
   kStatusEmptyWaitTimeout = 5,
   kStatusPeerArrivalTimeout = 6, // another GPU's arrival flag after a fused all-gather
+  // not waits: an index read from device memory that lies outside its table; the access was skipped
+  kStatusBadSlot = 7, // detail = token
+  kStatusBadPage = 8, // detail = sequence
 };
 
 __device__ __forceinline__ void report_status(uint32_t *status, uint32_t code, uint32_t detail) {

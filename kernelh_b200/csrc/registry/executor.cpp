@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstring>
+#include <iterator>
 
 namespace kh {
 
@@ -183,7 +184,7 @@ const char *Executor::wait_name(uint32_t code) {
   static const char *names[] = {"ok", "scan look-back wait", "TMA (full-stage) wait",
                                 "MMA (accumulator) wait", "epilogue wait", "empty-stage wait",
                                 "wait for another GPU's arrival flag (detail = its rank)"};
-  return code < 7 ? names[code] : "unknown wait";
+  return code < std::size(names) ? names[code] : "unknown wait";
 }
 
 Result<void> Executor::run(const std::string &kernel, const ShapeMap &shape,
@@ -232,6 +233,13 @@ Result<void> Executor::synchronize(StreamHandle stream) {
   (void)backend_->device_synchronize();
   const uint32_t code = host[0] ? host[0] : scan_host[0];
   const uint32_t detail = host[0] ? host[1] : scan_host[1];
+  // not waits: see kStatusBadSlot and kStatusBadPage in kernels/kh_device.cuh
+  if (code == 7)
+    return fail(kBadDeviceIndex, "a slot outside the cache was given for token " + std::to_string(detail) +
+                                     " (qk_norm_rope_append): its key and value were not stored");
+  if (code == 8)
+    return fail(kBadDeviceIndex, "a page table, length or query offset of sequence " + std::to_string(detail) +
+                                     " is out of range (paged_attention): its output is not defined");
   return fail(kDeviceTimeout, std::string("a device-side bounded wait ran out: ") + wait_name(code) + " (code " +
                                   std::to_string(code) + ", detail " + std::to_string(detail) +
                                   "); the kernel stopped and its output is incomplete");

@@ -7,6 +7,7 @@
 #pragma once
 
 #include "../runtime/objects.hpp"
+#include "kernelh_b200.h"
 #include "registry.hpp"
 
 #include <map>
@@ -146,5 +147,25 @@ Result<void> run_scan_lookback_probe(Executor &ex, const void *x, void *y, int64
 Result<void> run_attention_allgather(Executor &ex, const void *q, const void *k, const void *v,
                                      const std::vector<void *> &replicas, void *multicast, int rank,
                                      int world, int64_t slices, int64_t seq, StreamHandle stream);
+
+// qk_norm_rope_kernel.cpp. The check_ functions look at the arguments alone (no device needed); the
+// run_ functions take arguments that passed them.
+struct NormRopeCall {
+  kh_qk_norm_rope_args args;
+  kh_head_rows q_out, k_out;   // forward outputs, or the gradients of q and k
+  kh_head_rows dq_out, dk_out; // backward only
+  float *dq_weight = nullptr, *dk_weight = nullptr;
+  void *workspace = nullptr;
+  int64_t workspace_bytes = 0;
+  kh_head_rows v; // append only
+  const int64_t *slots = nullptr;
+  kh_paged_rows k_cache, v_cache;
+  int64_t num_pages = 0;
+  int32_t page_size = 0;
+  enum Kind { Forward, Backward, Append } kind = Forward;
+};
+int64_t qk_norm_rope_backward_workspace(int32_t head_dim);
+Result<void> check_qk_norm_rope(const char *entry, const NormRopeCall &call);
+Result<void> run_qk_norm_rope(Executor &ex, NormRopeCall call, StreamHandle stream);
 
 } // namespace kh

@@ -14,6 +14,8 @@ namespace kh {
 inline constexpr int kDriverUnavailable = 77;
 // A device-side bounded wait ran out (see csrc/kernels/kh_device.cuh).
 inline constexpr int kDeviceTimeout = 1001;
+// A kernel found an index in device memory outside its table and skipped the access.
+inline constexpr int kBadDeviceIndex = 1002;
 
 struct Error {
   int code = 0;
