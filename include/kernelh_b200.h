@@ -329,6 +329,51 @@ int kh_qk_norm_rope_append(kh_context *ctx, const kh_qk_norm_rope_args *args, kh
                            const int64_t *slots, kh_head_rows q_out, kh_paged_rows k_cache,
                            kh_paged_rows v_cache, int64_t num_pages, int32_t page_size, void *stream);
 
+/* Attention of new tokens over a paged cache, O = softmax(scale Q K^T + mask) V, for
+ * `batch` sequences of any lengths in one call: single new tokens (decoding), chunks of
+ * prompts, whole prompts, or a mixture. Sequence b has kv_len[b] keys, the last
+ * q_start[b + 1] - q_start[b] of which are its new tokens; those are the rows
+ * q_start[b] .. q_start[b + 1] - 1 of q and o (their keys and values are in the cache
+ * already). Key j of it is slot j % page_size of page page_table[b * table_stride +
+ * j / page_size]. Query t of n sees key j < kv when
+ *   causal: j <= kv - n + t (its own position and what lies before it),
+ *   window > 0: j > kv - n + t - window.
+ * A query that sees no key gives zeros (lse -inf). Query head h reads key/value head
+ * h / (q_heads / k_heads). lse (NULL: not wanted): log of the sum of exp, natural,
+ * [tokens, q_heads] fp32. Rows of o and lse behind the last sequence stay as they are.
+ * head_dim: a multiple of 8 up to 256. Rows of q, o and the cache start on 16-byte
+ * boundaries. page_size: any; pages may be shared between sequences. Slots that no
+ * query sees are not used, whatever they hold; a NaN or infinity in a value that some
+ * query sees reaches the queries that the mask keeps from it if they are worked on
+ * together (up to 256 neighbouring rows).
+ * q_start, kv_len and page_table are read on the device: a captured call follows their
+ * contents. max_q_len and max_kv_len only size the launch: larger lengths than these
+ * give right results, more slowly. q_start must not decrease nor exceed tokens, kv_len
+ * lie in 0 .. table_width * page_size, and pages in 0 .. num_pages - 1: what does not is
+ * not accessed, the sequence's output is not defined, and kh_synchronize reports it
+ * (1002). o must not overlap q or the cache. `workspace`: device memory of
+ * kh_paged_attention_workspace(args) bytes, 16-byte aligned, any contents, not shared
+ * with a call that may run at the same time. The same call gives the same bits. */
+typedef struct {
+  int32_t dtype, q_heads, k_heads, head_dim;
+  int64_t tokens; /* rows of q and o */
+  int32_t batch, max_q_len, max_kv_len, causal, window;
+  float scale;
+  kh_head_rows q, o;
+  float *lse;
+  kh_paged_rows k_cache, v_cache;
+  int64_t num_pages;
+  int32_t page_size, table_width;
+  const int32_t *page_table;
+  int64_t table_stride;
+  const int32_t *q_start, *kv_len;
+  void *workspace;
+  int64_t workspace_bytes;
+} kh_paged_attention_args;
+/* Reads dtype, heads, head_dim, tokens, batch, max_q_len and max_kv_len. */
+int64_t kh_paged_attention_workspace(const kh_paged_attention_args *args);
+int kh_paged_attention(kh_context *ctx, const kh_paged_attention_args *args, void *stream);
+
 /* The SM clock the last gemm launch of this context really ran at: block 0 of the
  * kernel counts its SM's cycles against the GPU's nanosecond timer over its whole
  * life; cycles / nanoseconds * 1000 = MHz under load (the management library's

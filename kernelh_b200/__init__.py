@@ -76,6 +76,16 @@ class QkNormRopeArgs(C.Structure):
                 ("inv_freq", C.c_void_p), ("positions", C.c_void_p)]
 
 
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("q_heads", C.c_int32), ("k_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("tokens", C.c_int64), ("batch", C.c_int32), ("max_q_len", C.c_int32), ("max_kv_len", C.c_int32),
+                ("causal", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("q", HeadRows), ("o", HeadRows),
+                ("lse", C.c_void_p), ("k_cache", PagedRows), ("v_cache", PagedRows), ("num_pages", C.c_int64),
+                ("page_size", C.c_int32), ("table_width", C.c_int32), ("page_table", C.c_void_p),
+                ("table_stride", C.c_int64), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -123,6 +133,9 @@ def _load() -> C.CDLL:
     L.kh_qk_norm_rope_backward_workspace.restype = i64
     L.kh_qk_norm_rope_backward.argtypes = [vp, rope, HeadRows, HeadRows, HeadRows, HeadRows, f32p, f32p, vp, i64, vp]
     L.kh_qk_norm_rope_append.argtypes = [vp, rope, HeadRows, vp, HeadRows, PagedRows, PagedRows, i64, C.c_int32, vp]
+    L.kh_paged_attention_workspace.argtypes = [C.POINTER(PagedAttentionArgs)]
+    L.kh_paged_attention_workspace.restype = i64
+    L.kh_paged_attention.argtypes = [vp, C.POINTER(PagedAttentionArgs), vp]
     L.kh_malloc.argtypes = [vp, C.c_size_t, C.POINTER(vp)]
     L.kh_free.argtypes = [vp, vp]
     L.kh_memcpy_h2d.argtypes = [vp, vp, vp, C.c_size_t]
@@ -485,6 +498,42 @@ class Context:
             self._h, a, self._rows(v, "v", k.shape, a.dtype), self._on_device(slots, "slots", "torch.int64", a.tokens),
             self._rows(q_out, "q_out", q.shape, a.dtype), self._cache(k_cache, "k_cache", shape, a.dtype),
             self._cache(v_cache, "v_cache", shape, a.dtype), pages, page_size, stream))
+
+    def paged_attention_workspace(self, q, k_cache, batch: int, max_q_len: int, max_kv_len: int) -> int:
+        """Bytes of device memory that `paged_attention` needs for such tensors and lengths."""
+        a = PagedAttentionArgs(_dtype_code(q, "q"), q.shape[1], k_cache.shape[2], q.shape[2], q.shape[0], batch, max_q_len,
+                               max_kv_len)
+        return int(lib.kh_paged_attention_workspace(a))
+
+    def paged_attention(self, q, k_cache, v_cache, page_table, q_start, kv_len, o, max_q_len, max_kv_len, workspace,
+                        scale=None, causal=True, window=0, lse=None, stream=None):
+        """Attention of new tokens over a paged cache. `q`, `o` [tokens, q_heads, head_dim] (float32, bfloat16 or
+        float16), `k_cache`, `v_cache` [pages, page_size, k_heads, head_dim], any strides but the last. Sequence b has
+        kv_len[b] keys on the pages page_table[b, :]; its new tokens, the last of those keys, are the rows
+        q_start[b] .. q_start[b + 1] - 1. `page_table` int32 [batch, width], `q_start` int32 [batch + 1], `kv_len` int32
+        [batch]: read on the device. `window`: a query sees its last `window` keys (0: all). `scale`: head_dim ** -0.5
+        when None. `lse` fp32 [tokens, q_heads] or None. `max_q_len`, `max_kv_len` size the launch. `workspace`: any
+        contiguous tensor of `paged_attention_workspace(...)` bytes."""
+        if q.dim() != 3 or k_cache.dim() != 4:
+            _refuse("'q' must be [tokens, heads, head_dim], 'k_cache' [pages, page_size, k_heads, head_dim]")
+        code = _dtype_code(q, "q")
+        tokens, q_heads, head_dim = q.shape
+        pages, page_size, k_heads, _ = k_cache.shape
+        if page_table.dim() != 2 or str(page_table.dtype) != "torch.int32" or page_table.stride(1) != 1:
+            _refuse("'page_table' must be int32 [batch, width] with contiguous rows")
+        if not page_table.is_cuda or page_table.get_device() != self._ordinal:
+            _refuse(f"'page_table' must be on device {self._ordinal} of this context, got {page_table.device}")
+        batch, width = page_table.shape
+        shape = (pages, page_size, k_heads, head_dim)
+        a = PagedAttentionArgs(
+            code, q_heads, k_heads, head_dim, tokens, batch, max_q_len, max_kv_len, 1 if causal else 0, window,
+            head_dim ** -0.5 if scale is None else scale, self._rows(q, "q", q.shape, code), self._rows(o, "o", q.shape, code),
+            None if lse is None else self._on_device(lse, "lse", "torch.float32", tokens * q_heads),
+            self._cache(k_cache, "k_cache", shape, code), self._cache(v_cache, "v_cache", shape, code), pages, page_size, width,
+            page_table.data_ptr(), page_table.stride(0), self._on_device(q_start, "q_start", "torch.int32", batch + 1),
+            self._on_device(kv_len, "kv_len", "torch.int32", batch), self._on_device(workspace, "workspace"),
+            workspace.numel() * workspace.element_size())
+        _check(lib.kh_paged_attention(self._h, a, stream))
 
     # ---- raw device memory -------------------------------------------------------
     def malloc(self, nbytes: int) -> int:

@@ -397,6 +397,19 @@ int kh_qk_norm_rope_append(kh_context *ctx, const kh_qk_norm_rope_args *args, kh
   return norm_rope(ctx, "kh_qk_norm_rope_append", c, stream);
 }
 
+int64_t kh_paged_attention_workspace(const kh_paged_attention_args *args) {
+  return args == nullptr ? 0 : kh::paged_attention_workspace(*args);
+}
+int kh_paged_attention(kh_context *ctx, const kh_paged_attention_args *args, void *stream) {
+  if (args == nullptr) return set_error(2, "kh_paged_attention: null arguments");
+  return guarded([&] {
+    if (auto r = kh::check_paged_attention(*args); !r) return set_error(r.error());
+    if (int rc = need_ctx(ctx)) return rc;
+    auto r = kh::run_paged_attention(*ctx->exec, *args, stream);
+    return r ? 0 : set_error(r.error());
+  });
+}
+
 int kh_malloc(kh_context *ctx, size_t bytes, void **out) {
   if (int rc = need_ctx(ctx)) return rc;
   if (out == nullptr) return set_error(2, "kh_malloc: null out pointer");

@@ -1,0 +1,446 @@
+// paged_attention: attention of new tokens over a paged cache, O = softmax(scale Q K^T + mask) V, for
+// sequences of any lengths side by side: decoding (one new token), chunks of a prompt, or both in one call.
+// fp32, bf16 or fp16; grouped key/value heads; causal and sliding-window masks; optional log-sum-exp.
+//
+// This file: the kernel for few rows per key/value head, and for types and head sizes that the tensor-memory
+// kernel does not take. A block of warps works on one item (see kh_paged.cuh) at a time, 16 rows of queries,
+// one m16 tile. Every warp streams its own 16 keys of each unit through a ring of its own (cp.async, no block
+// barrier inside an item) and keeps its own running maximum, sum and 16 x head_dim output in registers; the
+// warps are added up at the end of the item, through shared memory, in a fixed order.
+//   S = Q K^T and O += P V run as mma.sync m16n8k16 (16-bit types) or as three m16n8k8 tf32 products of
+//   hi/lo parts of 11 significant bits each (fp32; lo.lo is dropped: 2^-22 of a product).
+// HBM-bound at decoding: 4 rows x 128 values of queries cost 0.5 flop per byte of cache per row, far below
+// what any matrix unit needs; what counts is bytes in flight: two 16-key stages of keys and values per
+// warp, 8 warps per SM, are 128 KiB. Scores, softmax and sums are fp32; P is rounded to the values' type for
+// the second product (it is an operand of the 16-bit matrix instruction; 2^-9 of a probability in bf16), the
+// row sum is taken before that rounding; fp32 keeps P in hi/lo parts.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kh_paged.cuh"
+
+namespace {
+
+using khp::PagedParams;
+
+constexpr int kRows = 16;    // rows of an item
+constexpr int kKeys = 16;    // keys of a warp's step
+constexpr int kStages = 3;   // ring of a warp
+
+template <typename T, int kDim> struct Config {
+  static constexpr int kRowBytes = kDim * static_cast<int>(sizeof(T));
+  static constexpr int kWarps = kRowBytes <= 512 ? 4 : 2; // 3 stages of 16 keys and values per warp must fit
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kUnit = 64; // keys of a unit: the same for every type, so that the host can count
+  static constexpr int kSteps = kUnit / (kKeys * kWarps);
+  static constexpr int kPitch = kRowBytes + 16; // bytes between rows: ldmatrix and fp32 reads without bank conflicts
+  static constexpr int kTile = kKeys * kPitch;
+  static constexpr int kRing = kStages * 2 * kTile;
+  static constexpr int kSmem = kWarps * kRing;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// 16 bytes global -> shared; nothing is read and zeros are written when !valid
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo, both rounded to nearest at 11 significant bits (cut instead, the parts left over all have
+// one sign and add up: 1.6e-6 of a decoding step's output in 2-norm against 8e-7). (An infinity gives NaN, inf - inf.)
+__device__ __forceinline__ uint32_t round_tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo) {
+  hi = round_tf32(__uint_as_float(x));
+  lo = round_tf32(__uint_as_float(x) - __uint_as_float(hi));
+}
+template <int n> __device__ __forceinline__ void split_tf32(const uint32_t (&x)[n], uint32_t (&hi)[n], uint32_t (&lo)[n]) {
+#pragma unroll
+  for (int i = 0; i < n; ++i) split_tf32(x[i], hi[i], lo[i]);
+}
+__device__ __forceinline__ void mma8_fp32(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t b0, uint32_t b1) {
+  uint32_t h0, l0, h1, l1;
+  split_tf32(b0, h0, l0);
+  split_tf32(b1, h1, l1);
+  mma8_tf32(d, al, h0, h1);
+  mma8_tf32(d, ah, l0, l1);
+  mma8_tf32(d, ah, h0, h1);
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// The 16-row query tile as A fragments. 16-bit: k-step s holds rows (g, g + 8) x columns 16 s + 2c (+1) and
+// + 8; fp32: k-step s holds columns 8 s + c and + 4 (g = lane / 4, c = lane % 4). Zeros outside rows and head_dim.
+template <typename T, int kDim> struct Queries {
+  static constexpr bool k16 = sizeof(T) == 2;
+  static constexpr int kStepsK = k16 ? kDim / 16 : kDim / 8;
+  uint32_t a[kStepsK][4];
+  __device__ __forceinline__ void load(const PagedParams &P, const T *row0, const T *row1) {
+    const int c = threadIdx.x & 3;
+#pragma unroll
+    for (int s = 0; s < kStepsK; ++s) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const T *row = j & 1 ? row1 : row0;
+        const int col = k16 ? 16 * s + 2 * c + (j >> 1) * 8 : 8 * s + c + (j >> 1) * 4;
+        a[s][j] = row != nullptr && col < P.head_dim ? *reinterpret_cast<const uint32_t *>(row + col) : 0u;
+      }
+    }
+  }
+};
+
+// S (16 rows x 16 keys, two n8 tiles) of one tile of keys in shared memory
+template <typename T, int kDim>
+__device__ __forceinline__ void score_tile(const Queries<T, kDim> &q, uint32_t tile, float (&s)[2][4]) {
+  using Cfg = Config<T, kDim>;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
+  // matrices of one ldmatrix.x4: keys 0-7 and 8-15, each with the two 16-byte halves of the k-step
+  const uint32_t at = tile + ((lane & 7) + ((lane >> 4) << 3)) * Cfg::kPitch + ((lane >> 3) & 1) * 16;
+#pragma unroll
+  for (int k = 0; k < Queries<T, kDim>::kStepsK; ++k) {
+    uint32_t b[4];
+    ldsm4(b, at + k * 32);
+    if constexpr (sizeof(T) == 2) {
+      mma16<T>(s[0], q.a[k], b[0], b[1]);
+      mma16<T>(s[1], q.a[k], b[2], b[3]);
+    } else {
+      uint32_t hi[4], lo[4];
+      split_tf32(q.a[k], hi, lo);
+      mma8_fp32(s[0], hi, lo, b[0], b[1]);
+      mma8_fp32(s[1], hi, lo, b[2], b[3]);
+    }
+  }
+}
+
+// O += P V for one tile: p holds the probabilities in the score layout
+template <typename T, int kDim>
+__device__ __forceinline__ void value_tile(const float (&p)[2][4], uint32_t tile, float (&o)[kDim / 8][4]) {
+  using Cfg = Config<T, kDim>;
+  const int lane = threadIdx.x & 31;
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t a[4] = {pack<T>(p[0][0], p[0][1]), pack<T>(p[0][2], p[0][3]), pack<T>(p[1][0], p[1][1]), pack<T>(p[1][2], p[1][3])};
+    const uint32_t at = tile + (lane & 15) * Cfg::kPitch + (lane >> 4) * 16;
+#pragma unroll
+    for (int n = 0; n < kDim / 16; ++n) {
+      uint32_t b[4];
+      ldsm4_trans(b, at + n * 32);
+      mma16<T>(o[2 * n], a, b[0], b[1]);
+      mma16<T>(o[2 * n + 1], a, b[2], b[3]);
+    }
+  } else {
+    // k index c of the product stands for key 2c of its 8, c + 4 for key 2c + 1: the score layout as it is
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t a[4] = {__float_as_uint(p[t][0]), __float_as_uint(p[t][2]), __float_as_uint(p[t][1]), __float_as_uint(p[t][3])};
+      uint32_t hi[4], lo[4];
+      split_tf32(a, hi, lo);
+      const uint32_t at = tile + (8 * t + 2 * (lane & 3)) * Cfg::kPitch + (lane >> 2) * 4;
+#pragma unroll
+      for (int n = 0; n < kDim / 8; ++n) {
+        uint32_t b0, b1;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(b0) : "r"(at + n * 32) : "memory");
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(b1) : "r"(at + n * 32 + Cfg::kPitch) : "memory");
+        mma8_fp32(o[n], hi, lo, b0, b1);
+      }
+    }
+  }
+}
+
+template <typename T, int kDim> __device__ __forceinline__ void attention_body(const PagedParams &P) {
+  using Cfg = Config<T, kDim>;
+  constexpr int kThreads = Cfg::kThreads, kWarps = Cfg::kWarps, kUnit = Cfg::kUnit;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ khp::LineScratch<kThreads> scratch;
+  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t ring = smem_addr(smem) + warp * Cfg::kRing;
+  if (P.head_dim < kDim) { // columns that no copy writes count as zeros
+    for (int i = threadIdx.x * 16; i < Cfg::kSmem; i += kThreads * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  khd::grid_dependency_wait();
+  khd::grid_dependents_may_launch();
+  const khp::Line line = khp::measure_line<kThreads, kRows, kUnit>(P, scratch);
+  const int w = blockIdx.x;
+  if (w >= line.workers) return;
+  int64_t at = khp::stretch(line, w);
+  const int64_t until = khp::stretch(line, w + 1);
+  const int64_t from = at;
+  int b;
+  int64_t start;
+  khp::locate<kThreads, kRows, kUnit>(P, at, scratch, b, start);
+  khp::Sequence s = khp::sequence<kRows, kUnit>(P, b);
+
+  const int chunks_per_row = P.head_dim * static_cast<int>(sizeof(T)) / 16; // 16-byte pieces that exist
+  while (at < until) {
+    int64_t size = static_cast<int64_t>(s.blocks) * s.units * P.k_heads;
+    while (at >= start + size) { // on to the next sequence that has rows
+      start += size;
+      s = khp::sequence<kRows, kUnit>(P, ++b);
+      size = static_cast<int64_t>(s.blocks) * s.units * P.k_heads;
+    }
+    const int64_t item = (at - start) / s.units;
+    const int64_t begin = start + item * s.units, end = begin + s.units;
+    const int h = static_cast<int>(item / s.blocks);
+    const int block = khp::block_of(static_cast<int>(item - static_cast<int64_t>(h) * s.blocks), s.blocks);
+    const int unit0 = static_cast<int>(at - begin), unit1 = static_cast<int>((until < end ? until : end) - begin);
+    const int row0 = block * kRows, rows_here = min(kRows, s.rows - row0);
+    // keys that rows of this block see, and the part of them in this stretch
+    const int t_first = row0 / P.group, t_last = (row0 + rows_here - 1) / P.group;
+    const int past = s.kv - s.tokens; // position of token 0 (negative: its first tokens see nothing)
+    const int hi_key = P.causal ? max(0, min(s.kv, past + t_last + 1)) : s.kv;
+    const int64_t lo_window = P.window > 0 ? static_cast<int64_t>(past) + t_first - P.window + 1 : 0;
+    const int lo_key = lo_window > 0 ? static_cast<int>(min(lo_window, static_cast<int64_t>(s.kv))) : 0;
+    const int key_a = max((s.first_unit + unit0) * kUnit, lo_key / kUnit * kUnit);
+    const int key_b = static_cast<int>(min(static_cast<int64_t>(s.first_unit + unit1) * kUnit, static_cast<int64_t>(hi_key)));
+
+    // this lane's two rows: their queries and the keys they see
+    const int g = lane >> 2;
+    int see_lo[2], see_hi[2];
+    const T *q_row[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = row0 + g + 8 * i;
+      const bool real = r < s.rows;
+      const int t = real ? r / P.group : 0, head = h * P.group + (real ? r - t * P.group : 0);
+      q_row[i] = real ? reinterpret_cast<const T *>(P.q) + (s.q0 + t) * P.q_token + head * P.q_head : nullptr;
+      see_hi[i] = !real ? -1 : P.causal ? past + t : s.kv - 1;
+      const int64_t first = P.window > 0 ? static_cast<int64_t>(past) + t - P.window + 1 : 0;
+      see_lo[i] = static_cast<int>(first > 0 ? first : 0);
+    }
+    Queries<T, kDim> q;
+    q.load(P, q_row[0], q_row[1]);
+
+    float o[kDim / 8][4];
+#pragma unroll
+    for (int n = 0; n < kDim / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    const int32_t *table = P.table + b * P.table_stride;
+    const char *k_base = P.k + static_cast<int64_t>(h) * P.k_head * sizeof(T), *v_base = P.v + static_cast<int64_t>(h) * P.v_head * sizeof(T);
+    const int steps = key_b > key_a ? ((key_b - key_a + kUnit - 1) / kUnit) * Cfg::kSteps : 0;
+    const auto key_of = [&](int i) { return key_a + (i / Cfg::kSteps) * kUnit + (i % Cfg::kSteps * kWarps + warp) * kKeys; };
+    // lane r < 16 looks up the page of row r one step ahead of its use
+    int page_next = 0;
+    const auto look_up = [&](int i) {
+      const int key = key_of(i) + (lane & 15);
+      page_next = i < steps && key < key_b ? __ldg(table + key / P.page_size) : 0;
+    };
+    const auto issue = [&](int i) {
+      if (i < steps && key_of(i) < key_b) {
+        const int key0 = key_of(i), key = key0 + (lane & 15);
+        bool good = key < key_b && key >= lo_key; // evicted keys before every row's window are not read
+        int page = page_next;
+        if (good && (page < 0 || page >= P.num_pages)) {
+          khd::report_status(P.status, khd::kStatusBadPage, static_cast<uint32_t>(b));
+          good = false;
+        }
+        const int slot = key % P.page_size;
+        const int64_t k_off = good ? (page * P.k_page + slot * P.k_slot) * static_cast<int64_t>(sizeof(T)) : -1;
+        const int64_t v_off = good ? (page * P.v_page + slot * P.v_slot) * static_cast<int64_t>(sizeof(T)) : -1;
+        const uint32_t k_tile = ring + (i % kStages) * 2 * Cfg::kTile, v_tile = k_tile + Cfg::kTile;
+        constexpr int kChunks = Cfg::kRowBytes / 16;
+#pragma unroll
+        for (int j = 0; j < kKeys * kChunks / 32; ++j) {
+          const int idx = j * 32 + lane, row = idx / kChunks, c = idx % kChunks;
+          const int64_t ko = __shfl_sync(0xffffffffu, k_off, row), vo = __shfl_sync(0xffffffffu, v_off, row);
+          if (c < chunks_per_row) {
+            copy16(k_tile + row * Cfg::kPitch + c * 16, ko >= 0 ? k_base + ko + c * 16 : k_base, ko >= 0);
+            copy16(v_tile + row * Cfg::kPitch + c * 16, vo >= 0 ? v_base + vo + c * 16 : v_base, vo >= 0);
+          }
+        }
+      }
+      copy_commit();
+      look_up(i + 1);
+    };
+    look_up(0);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+    for (int i = 0; i < steps; ++i) {
+      __syncwarp(); // every lane is done with the slot that is refilled now
+      issue(i + kStages - 1);
+      copy_wait<kStages - 1>();
+      __syncwarp();
+      const int key0 = key_of(i);
+      if (key0 >= key_b) continue;
+      const uint32_t k_tile = ring + (i % kStages) * 2 * Cfg::kTile;
+      float sc[2][4];
+      score_tile<T, kDim>(q, k_tile, sc);
+      float top[2] = {m[0], m[1]};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = key0 + 8 * t + 2 * (lane & 3) + (j & 1), i2 = j >> 1;
+          const bool seen = key <= see_hi[i2] && key >= see_lo[i2];
+          sc[t][j] = seen ? sc[t][j] * P.scale_log2 : -INFINITY;
+          top[i2] = fmaxf(top[i2], sc[t][j]);
+        }
+#pragma unroll
+      for (int i2 = 0; i2 < 2; ++i2) {
+        top[i2] = fmaxf(top[i2], __shfl_xor_sync(0xffffffffu, top[i2], 1));
+        top[i2] = fmaxf(top[i2], __shfl_xor_sync(0xffffffffu, top[i2], 2));
+      }
+      if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+#pragma unroll
+        for (int i2 = 0; i2 < 2; ++i2) {
+          const float f = exp2f(m[i2] - (top[i2] == -INFINITY ? 0.f : top[i2]));
+          m[i2] = top[i2];
+          l[i2] *= f;
+#pragma unroll
+          for (int n = 0; n < kDim / 8; ++n) {
+            o[n][2 * i2] *= f;
+            o[n][2 * i2 + 1] *= f;
+          }
+        }
+      }
+      // a row that has seen no key yet keeps max -inf; its exponentials are taken against 0 and are all 0
+      const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sc[t][j] = exp2f(sc[t][j] - ref[j >> 1]);
+          l[j >> 1] += sc[t][j];
+        }
+      value_tile<T, kDim>(sc, k_tile + Cfg::kTile, o);
+    }
+
+    // the warps' rows are added up: the rings are drained and serve as scratch
+    copy_wait<0>();
+#pragma unroll
+    for (int i2 = 0; i2 < 2; ++i2) {
+      l[i2] += __shfl_xor_sync(0xffffffffu, l[i2], 1);
+      l[i2] += __shfl_xor_sync(0xffffffffu, l[i2], 2);
+      if ((lane & 3) == 0) {
+        s_m[warp][g + 8 * i2] = m[i2];
+        s_l[warp][g + 8 * i2] = l[i2];
+      }
+    }
+    __syncthreads();
+    constexpr int kPitchF = kDim + 4;
+    float *mine = reinterpret_cast<float *>(smem + warp * Cfg::kRing);
+#pragma unroll
+    for (int i2 = 0; i2 < 2; ++i2) {
+      float top = s_m[0][g + 8 * i2];
+#pragma unroll
+      for (int x = 1; x < kWarps; ++x) top = fmaxf(top, s_m[x][g + 8 * i2]);
+      const float f = exp2f(m[i2] - (top == -INFINITY ? 0.f : top));
+#pragma unroll
+      for (int n = 0; n < kDim / 8; ++n)
+        *reinterpret_cast<float2 *>(mine + (g + 8 * i2) * kPitchF + n * 8 + 2 * (lane & 3)) = make_float2(o[n][2 * i2] * f, o[n][2 * i2 + 1] * f);
+    }
+    __syncthreads();
+    const bool whole = unit0 == 0 && unit1 == s.units;
+    const int64_t part = begin < from ? 2 * static_cast<int64_t>(w) : 2 * static_cast<int64_t>(w) + 1;
+    for (int i = threadIdx.x; i < rows_here * (kDim / 4); i += kThreads) {
+      const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
+      float top = s_m[0][r];
+#pragma unroll
+      for (int x = 1; x < kWarps; ++x) top = fmaxf(top, s_m[x][r]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        sum += s_l[x][r] * exp2f(s_m[x][r] - ref);
+        const float4 y = *reinterpret_cast<const float4 *>(smem + x * Cfg::kRing + (r * kPitchF + c) * 4);
+        v[0] += y.x, v[1] += y.y, v[2] += y.z, v[3] += y.w;
+      }
+      if (!whole) {
+        *reinterpret_cast<float4 *>(P.partial_o + (part * kRows + r) * kDim + c) = make_float4(v[0], v[1], v[2], v[3]);
+        if (c == 0) P.partial_ml[part * kRows + r] = make_float2(top, sum);
+        continue;
+      }
+      const int t = (row0 + r) / P.group, head = h * P.group + (row0 + r) - t * P.group;
+      const float inv = 1.f / sum;
+      if (c < P.head_dim) {
+        T *dst = reinterpret_cast<T *>(P.o) + (s.q0 + t) * P.o_token + head * P.o_head + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = sum != 0.f ? v[j] * inv : 0.f; // a row that sees no key: zeros
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+        else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]));
+      }
+      if (c == 0 && P.lse != nullptr)
+        P.lse[static_cast<int64_t>(s.q0 + t) * P.q_heads + head] = sum != 0.f ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+    }
+    __syncthreads(); // the scratch becomes rings again
+    if (P.head_dim < kDim) { // and their unwritten columns zeros
+      for (int i = threadIdx.x * 16; i < Cfg::kSmem; i += kThreads * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
+      __syncthreads();
+    }
+    at = begin + unit1;
+  }
+}
+
+template <typename T, int kDim> __device__ __forceinline__ void combine(const PagedParams &P) {
+  khp::combine_body<T, 128, kRows, Config<T, kDim>::kUnit, kDim>(P, [&](int token, int head, int c, float v) {
+    reinterpret_cast<T *>(P.o)[token * P.o_token + head * P.o_head + c] = from_float<T>(v);
+  });
+}
+
+} // namespace
+
+#define KH_PAGED(suffix, T, dim)                                                                                              \
+  extern "C" __global__ void __launch_bounds__(Config<T, dim>::kThreads)                                                      \
+  paged_attention_##suffix##_##dim(const __grid_constant__ PagedParams P) { attention_body<T, dim>(P); }                      \
+  extern "C" __global__ void __launch_bounds__(128) paged_attention_combine_##suffix##_##dim(                                 \
+      const __grid_constant__ PagedParams P) { combine<T, dim>(P); }
+
+KH_PAGED(f32, float, 64)
+KH_PAGED(f32, float, 128)
+KH_PAGED(f32, float, 256)
+KH_PAGED(bf16, __nv_bfloat16, 64)
+KH_PAGED(bf16, __nv_bfloat16, 128)
+KH_PAGED(bf16, __nv_bfloat16, 256)
+KH_PAGED(f16, __half, 64)
+KH_PAGED(f16, __half, 128)
+KH_PAGED(f16, __half, 256)

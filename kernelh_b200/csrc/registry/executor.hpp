@@ -168,4 +168,9 @@ int64_t qk_norm_rope_backward_workspace(int32_t head_dim);
 Result<void> check_qk_norm_rope(const char *entry, const NormRopeCall &call);
 Result<void> run_qk_norm_rope(Executor &ex, NormRopeCall call, StreamHandle stream);
 
+// paged_attention_kernel.cpp
+int64_t paged_attention_workspace(const kh_paged_attention_args &args);
+Result<void> check_paged_attention(const kh_paged_attention_args &args);
+Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args args, StreamHandle stream);
+
 } // namespace kh

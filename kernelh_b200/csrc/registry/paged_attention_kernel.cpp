@@ -1,0 +1,181 @@
+// Argument checks and launches of attention over a paged cache (kernels/paged_attention.cu). A typed entry
+// point only: the registry's launch by name takes fp32 buffers of one layout.
+#include "executor.hpp"
+
+#include <climits>
+#include <cmath>
+#include <string>
+
+namespace kh {
+namespace {
+
+constexpr int kRows = 16, kUnit = 64; // kernels/paged_attention.cu
+constexpr int kMinUnits = 2;          // keys per worker below which more workers cost more than they bring: 128
+constexpr long kMaxSms = 160;         // workspaces are sized for at most this many SMs
+
+int element_size(int32_t dtype) { return dtype == KH_F32 ? 4 : 2; }
+int padded_dim(int32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+// Layout shared with kernels/kh_paged.cuh.
+struct PagedParams {
+  const void *q;
+  int64_t q_token, q_head;
+  void *o;
+  int64_t o_token, o_head;
+  const void *k;
+  int64_t k_page, k_slot, k_head;
+  const void *v;
+  int64_t v_page, v_slot, v_head;
+  const int32_t *table;
+  int64_t table_stride;
+  const int32_t *q_start, *kv_len;
+  float *lse, *partial_o;
+  void *partial_ml;
+  uint32_t *status;
+  int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, table_width, num_pages;
+  int32_t causal, window;
+  int32_t workers, min_units;
+  int32_t rows_above, rows_upto;
+  float scale_log2;
+};
+static_assert(sizeof(PagedParams) <= LaunchArgs::kMaxStructBytes);
+
+// Blocks of the kernel that an SM holds: by shared memory (a ring of 3 x 32 padded rows per warp) and registers.
+struct Shape {
+  int dim, warps, per_sm;
+  size_t smem;
+};
+Shape kernel_shape(int32_t dtype, int32_t head_dim) {
+  Shape s{};
+  s.dim = padded_dim(head_dim);
+  const int row_bytes = s.dim * element_size(dtype);
+  s.warps = row_bytes <= 512 ? 4 : 2;
+  s.per_sm = row_bytes <= 128 ? 3 : row_bytes <= 256 ? 2 : 1;
+  s.smem = static_cast<size_t>(s.warps) * 3 * 2 * 16 * (row_bytes + 16);
+  return s;
+}
+
+// Grows with `sms` and with every length: the workspace, counted for kMaxSms, covers any device's launch.
+int64_t worker_count(const kh_paged_attention_args &a, const Shape &s, long sms) {
+  const int64_t group = a.q_heads / a.k_heads;
+  const int64_t items = (a.tokens * group / kRows + a.batch) * a.k_heads; // at most
+  const int64_t units = std::max<int64_t>(1, (static_cast<int64_t>(std::max(a.max_kv_len, 1)) + kUnit - 1) / kUnit);
+  const int64_t most = s.per_sm * std::min(sms, kMaxSms);
+  return std::min<int64_t>(most, std::max<int64_t>(1, (items * units + kMinUnits - 1) / kMinUnits));
+}
+int64_t workspace_for(const Shape &s, int64_t workers) { return 2 * workers * kRows * (s.dim * 4 + 8); }
+
+std::string check_stride(const char *name, const void *data, std::initializer_list<std::pair<int64_t, int64_t>> strides, int32_t head_dim,
+                         int size, bool output) {
+  if (data == nullptr) return std::string("buffer '") + name + "' is null";
+  bool aligned = reinterpret_cast<uintptr_t>(data) % 16 == 0;
+  for (const auto &[stride, count] : strides) {
+    if (count <= 1) continue;
+    aligned = aligned && stride * size % 16 == 0;
+    if (output && std::abs(stride) < head_dim) return std::string("rows of output '") + name + "' overlap (a stride below head_dim)";
+  }
+  if (!aligned) return std::string("rows of '") + name + "' do not start on 16-byte boundaries (pass an aligned copy)";
+  return "";
+}
+
+} // namespace
+
+int64_t paged_attention_workspace(const kh_paged_attention_args &a) {
+  if (a.q_heads < 1 || a.k_heads < 1 || a.head_dim < 1 || a.head_dim > 256 || a.tokens < 0 || a.batch < 0) return 0;
+  const Shape s = kernel_shape(a.dtype, a.head_dim);
+  return workspace_for(s, worker_count(a, s, kMaxSms));
+}
+
+Result<void> check_paged_attention(const kh_paged_attention_args &a) {
+  const auto refuse = [&](const std::string &why) { return fail(2, "kh_paged_attention: " + why); };
+  if (a.dtype != KH_F32 && a.dtype != KH_BF16 && a.dtype != KH_F16)
+    return refuse("dtype must be KH_F32, KH_BF16 or KH_F16 (got " + std::to_string(a.dtype) + ")");
+  if (a.q_heads < 1 || a.k_heads < 1 || a.q_heads > (1 << 20) || a.q_heads % a.k_heads != 0)
+    return refuse("q_heads must be a positive multiple of k_heads, at most 2^20 (got " + std::to_string(a.q_heads) + " and " +
+                  std::to_string(a.k_heads) + ")");
+  if (a.head_dim < 8 || a.head_dim > 256 || a.head_dim % 8 != 0)
+    return refuse("head_dim must be a multiple of 8 up to 256 (got " + std::to_string(a.head_dim) + ")");
+  if (a.tokens < 0 || a.tokens * (a.q_heads / a.k_heads) > INT_MAX - 1024)
+    return refuse("tokens * q_heads / k_heads must lie in 0 .. 2^31 - 1025");
+  if (a.batch < 0 || a.max_q_len < 0 || a.max_kv_len < 0) return refuse("batch, max_q_len and max_kv_len must not be negative");
+  if (a.causal != 0 && a.causal != 1) return refuse("causal must be 0 or 1");
+  if (a.window < 0) return refuse("window must not be negative (0: none)");
+  if (!std::isfinite(a.scale)) return refuse("scale must be finite");
+  if (a.num_pages < 1 || a.num_pages > INT_MAX || a.page_size < 1 || a.page_size > (1 << 24))
+    return refuse("num_pages must lie in 1 .. 2^31 - 1 and page_size in 1 .. 2^24");
+  if (a.table_width < 0 || static_cast<int64_t>(a.table_width) * a.page_size > INT_MAX - 1024)
+    return refuse("a page table row must hold at most 2^31 - 1025 slots");
+  if (a.batch > 1 && std::abs(a.table_stride) < a.table_width) return refuse("rows of the page table overlap");
+  if (a.tokens == 0 || a.batch == 0) return {};
+  const int size = element_size(a.dtype);
+  std::string why = check_stride("q", a.q.data, {{a.q.token_stride, a.tokens}, {a.q.head_stride, a.q_heads}}, a.head_dim, size, false);
+  if (why.empty()) why = check_stride("o", a.o.data, {{a.o.token_stride, a.tokens}, {a.o.head_stride, a.q_heads}}, a.head_dim, size, true);
+  for (const auto &[name, c] : {std::pair<const char *, kh_paged_rows>{"k_cache", a.k_cache}, {"v_cache", a.v_cache}})
+    if (why.empty())
+      why = check_stride(name, c.data, {{c.page_stride, a.num_pages}, {c.slot_stride, a.page_size}, {c.head_stride, a.k_heads}}, a.head_dim,
+                         size, false);
+  for (const auto &[name, p] : {std::pair<const char *, const void *>{"page_table", a.page_table}, {"q_start", a.q_start}, {"kv_len", a.kv_len}, {"lse", a.lse}}) {
+    if (!why.empty()) break;
+    if (p == nullptr && name != std::string("lse") && !(name == std::string("page_table") && a.table_width == 0))
+      why = std::string("buffer '") + name + "' is null";
+    else if (reinterpret_cast<uintptr_t>(p) % 4 != 0) why = std::string("buffer '") + name + "' is not 4-byte aligned";
+  }
+  if (why.empty() && a.q.data == a.o.data) why = "o must not be q itself";
+  if (!why.empty()) return refuse(why);
+  const int64_t need = paged_attention_workspace(a);
+  if (a.workspace == nullptr || a.workspace_bytes < need)
+    return refuse("the workspace must have " + std::to_string(need) + " bytes (got " +
+                  std::to_string(a.workspace == nullptr ? 0 : a.workspace_bytes) + ")");
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) return refuse("the workspace is not 16-byte aligned");
+  return {};
+}
+
+Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, StreamHandle stream) {
+  if (a.tokens == 0 || a.batch == 0) return {};
+  long sms = query_cu_count(ex.limits());
+  if (sms <= 0) sms = 148;
+  const Shape s = kernel_shape(a.dtype, a.head_dim);
+  const int64_t workers = worker_count(a, s, sms);
+  PagedParams p{};
+  const auto stride = [](int64_t v, int64_t count) { return count > 1 ? v : 0; };
+  p.q = a.q.data, p.q_token = stride(a.q.token_stride, a.tokens), p.q_head = stride(a.q.head_stride, a.q_heads);
+  p.o = a.o.data, p.o_token = stride(a.o.token_stride, a.tokens), p.o_head = stride(a.o.head_stride, a.q_heads);
+  p.k = a.k_cache.data, p.k_page = stride(a.k_cache.page_stride, a.num_pages), p.k_slot = stride(a.k_cache.slot_stride, a.page_size);
+  p.v = a.v_cache.data, p.v_page = stride(a.v_cache.page_stride, a.num_pages), p.v_slot = stride(a.v_cache.slot_stride, a.page_size);
+  p.k_head = stride(a.k_cache.head_stride, a.k_heads), p.v_head = stride(a.v_cache.head_stride, a.k_heads);
+  p.table = a.page_table, p.table_stride = a.batch > 1 ? a.table_stride : 0;
+  p.q_start = a.q_start, p.kv_len = a.kv_len;
+  p.lse = a.lse;
+  p.partial_o = static_cast<float *>(a.workspace);
+  p.partial_ml = static_cast<char *>(a.workspace) + 2 * workers * kRows * s.dim * 4;
+  p.status = ex.status_word();
+  p.tokens = static_cast<int32_t>(a.tokens), p.batch = a.batch, p.q_heads = a.q_heads, p.k_heads = a.k_heads;
+  p.group = a.q_heads / a.k_heads, p.head_dim = a.head_dim;
+  p.page_size = a.page_size, p.table_width = a.table_width, p.num_pages = static_cast<int32_t>(a.num_pages);
+  p.causal = a.causal, p.window = a.window;
+  p.workers = static_cast<int32_t>(workers), p.min_units = kMinUnits;
+  p.rows_above = 0, p.rows_upto = INT_MAX;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  const std::string suffix = std::string(a.dtype == KH_F32 ? "f32_" : a.dtype == KH_BF16 ? "bf16_" : "f16_") + std::to_string(s.dim);
+  const auto launch = [&](const std::string &entry, LaunchDims grid, unsigned threads, size_t smem) -> Result<void> {
+    LaunchStep step;
+    step.entry = entry;
+    step.grid = grid;
+    step.block = {threads, 1, 1};
+    step.dynamic_smem = smem;
+    step.overlap_tail = true;
+    step.param_count = 1;
+    LaunchArgs args;
+    args.add_struct_bytes(&p, sizeof p);
+    auto fn = ex.function("paged_attention", entry);
+    if (!fn) return std::unexpected(fn.error());
+    return ex.launch(*fn, step, args, stream);
+  };
+  if (auto r = launch("paged_attention_" + suffix, {static_cast<unsigned>(workers), 1, 1}, 32u * s.warps, s.smem); !r) return r;
+  if (workers == 1) return {};
+  // an item is split where a worker's stretch begins inside it: one row of blocks per such place
+  const int64_t rows = std::min<int64_t>(kRows, a.tokens * p.group);
+  return launch("paged_attention_combine_" + suffix, {static_cast<unsigned>(workers - 1), static_cast<unsigned>(rows), 1}, 128, 0);
+}
+
+} // namespace kh
