@@ -35,7 +35,7 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 KERNELS = ["vecadd", "fused_gelu", "scan", "softmax", "layernorm", "gemm", "attention"]
 # code objects: one per kernel template, then those behind typed entry points only
-IMAGES = KERNELS + ["qk_norm_rope", "paged_attention"]
+IMAGES = KERNELS + ["qk_norm_rope", "paged_attention", "paged_attention_chunk"]
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = NVCC_ARCH + ["-lineinfo", "-O3", "-std=c++17"]
 CXX = "g++"  # plain g++ from PATH: an inherited CXX may be a wrapper without C++23 support

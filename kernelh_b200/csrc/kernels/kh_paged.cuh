@@ -151,50 +151,63 @@ __device__ __forceinline__ void locate(const PagedParams &P, int64_t at, LineScr
   __syncthreads();
 }
 
-// Adds up the partial rows of one item: block (w, y) takes row y of the item that worker w's stretch
-// begins inside of, if no earlier stretch does. Its warps take every kThreads / 32-th part each with a
-// running maximum and are added up in order.
+// The item that worker w's stretch (w > 0) begins inside of, if no earlier stretch does, and its parts:
+// part 0 in slot 2 (w - 1) + 1, part p in slot 2 (w - 1 + p).
+struct Split {
+  Sequence s;
+  int h, row0, w, parts; // parts 0: nothing to add up here
+  __device__ __forceinline__ int64_t slot(int p) const { return 2 * static_cast<int64_t>(w - 1 + p) + (p == 0 ? 1 : 0); }
+};
+template <int kThreads, int kRows, int kUnit> __device__ __forceinline__ Split find_split(const PagedParams &P, LineScratch<kThreads> &scratch) {
+  Split x{};
+  const Line line = measure_line<kThreads, kRows, kUnit>(P, scratch);
+  x.w = blockIdx.x + 1;
+  if (x.w >= line.workers) return x;
+  const int64_t at = stretch(line, x.w);
+  int b;
+  int64_t start;
+  locate<kThreads, kRows, kUnit>(P, at, scratch, b, start);
+  x.s = sequence<kRows, kUnit>(P, b);
+  const int64_t item = (at - start) / x.s.units; // head * blocks + place of the row block
+  const int64_t begin = start + item * x.s.units, end = begin + x.s.units;
+  if (begin == at || begin < stretch(line, x.w - 1)) return x; // nothing split here, or an earlier block's
+  x.h = static_cast<int>(item / x.s.blocks);
+  x.row0 = block_of(static_cast<int>(item - static_cast<int64_t>(x.h) * x.s.blocks), x.s.blocks) * kRows;
+  int last = x.w; // the last worker with a part
+  while (last + 1 < line.workers && stretch(line, last + 1) < end) ++last;
+  x.parts = last - x.w + 2;
+  return x;
+}
+
+// Adds up the parts of one row, for items with few rows and many parts: block (w - 1, y) takes row y of w's
+// item. Its warps take every kThreads / 32-th part each with a running maximum and are added up in order.
 template <typename T, int kThreads, int kRows, int kUnit, int kDim, typename Store>
 __device__ __forceinline__ void combine_body(const PagedParams &P, Store store) {
   __shared__ LineScratch<kThreads> scratch;
   __shared__ float s_row[kThreads / 32][kDim];
   __shared__ float2 s_ml[kThreads / 32];
   khd::grid_dependency_wait();
-  const Line line = measure_line<kThreads, kRows, kUnit>(P, scratch);
-  const int w = blockIdx.x + 1;
-  if (w >= line.workers) return;
-  const int64_t at = stretch(line, w);
-  int b;
-  int64_t start;
-  locate<kThreads, kRows, kUnit>(P, at, scratch, b, start);
-  const Sequence s = sequence<kRows, kUnit>(P, b);
-  const int64_t item = (at - start) / s.units; // head * blocks + place of the row block
-  const int64_t begin = start + item * s.units, end = begin + s.units;
-  if (begin == at || begin < stretch(line, w - 1)) return; // nothing split here, or an earlier block's
-  const int h = static_cast<int>(item / s.blocks);
-  const int block = block_of(static_cast<int>(item - static_cast<int64_t>(h) * s.blocks), s.blocks);
-  const int row = block * kRows + static_cast<int>(blockIdx.y);
-  if (static_cast<int>(blockIdx.y) >= kRows || row >= s.rows) return;
-  int last = w; // the last worker with a part
-  while (last + 1 < line.workers && stretch(line, last + 1) < end) ++last;
-  const int parts = last - w + 2;
+  const Split x = find_split<kThreads, kRows, kUnit>(P, scratch);
+  const Sequence &s = x.s;
+  const int row = x.row0 + static_cast<int>(blockIdx.y), h = x.h, parts = x.parts;
+  if (parts == 0 || static_cast<int>(blockIdx.y) >= kRows || row >= s.rows) return;
   constexpr int kWarps = kThreads / 32, kPer = kDim / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float m = -INFINITY, l = 0.f, acc[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
   for (int p = warp; p < parts; p += kWarps) {
-    const int64_t slot = p == 0 ? 2 * static_cast<int64_t>(w - 1) + 1 : 2 * static_cast<int64_t>(w - 1 + p);
+    const int64_t slot = x.slot(p);
     const float2 ml = P.partial_ml[slot * kRows + blockIdx.y];
     const float *src = P.partial_o + (slot * kRows + blockIdx.y) * kDim + lane * kPer;
-    float x[kPer];
+    float y[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i] = src[i];
+    for (int i = 0; i < kPer; ++i) y[i] = src[i];
     const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
     const float f_old = exp2f(m - ref), f_new = exp2f(ml.x - ref);
     l = l * f_old + ml.y * f_new;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * f_old + x[i] * f_new;
+    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * f_old + y[i] * f_new;
     m = m_new;
   }
 #pragma unroll
@@ -220,6 +233,44 @@ __device__ __forceinline__ void combine_body(const PagedParams &P, Store store) 
   }
   if (threadIdx.x == 0 && P.lse != nullptr)
     P.lse[static_cast<int64_t>(token) * P.q_heads + head] = sum != 0.f ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+}
+
+// The same for items with many rows, which have few parts: block (w - 1, y) takes the rows y * 32 .. + 31 of w's
+// item, a warp takes whole rows and goes through their parts in order.
+template <int kThreads, int kRows, int kUnit, int kDim, typename Store>
+__device__ __forceinline__ void combine_rows(const PagedParams &P, Store store) {
+  __shared__ LineScratch<kThreads> scratch;
+  khd::grid_dependency_wait();
+  const Split x = find_split<kThreads, kRows, kUnit>(P, scratch);
+  if (x.parts == 0) return;
+  constexpr int kPer = kDim / 32, kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = warp; i < 32; i += kWarps) {
+    const int in_block = static_cast<int>(blockIdx.y) * 32 + i, row = x.row0 + in_block;
+    if (in_block >= kRows || row >= x.s.rows) return;
+    float m = -INFINITY, l = 0.f, acc[kPer];
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
+    for (int p = 0; p < x.parts; ++p) {
+      const int64_t at = x.slot(p) * kRows + in_block;
+      const float2 ml = P.partial_ml[at];
+      float y[kPer];
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) y[c] = P.partial_o[at * kDim + c * 32 + lane];
+      const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
+      const float f_old = exp2f(m - ref), f_new = exp2f(ml.x - ref);
+      l = l * f_old + ml.y * f_new;
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) acc[c] = acc[c] * f_old + y[c] * f_new;
+      m = m_new;
+    }
+    const int token = x.s.q0 + row / P.group, head = x.h * P.group + row % P.group;
+#pragma unroll
+    for (int c = 0; c < kPer; ++c)
+      if (c * 32 + lane < P.head_dim) store(token, head, c * 32 + lane, l != 0.f ? acc[c] / l : 0.f);
+    if (lane == 0 && P.lse != nullptr)
+      P.lse[static_cast<int64_t>(token) * P.q_heads + head] = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+  }
 }
 
 } // namespace khp

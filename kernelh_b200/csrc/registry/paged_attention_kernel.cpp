@@ -1,5 +1,6 @@
-// Argument checks and launches of attention over a paged cache (kernels/paged_attention.cu). A typed entry
-// point only: the registry's launch by name takes fp32 buffers of one layout.
+// Argument checks and launches of attention over a paged cache: kernels/paged_attention.cu for few rows per
+// key/value head, kernels/paged_attention_chunk.cu for many. A typed entry point only: the registry's launch by
+// name takes fp32 buffers of one layout.
 #include "executor.hpp"
 
 #include <climits>
@@ -9,8 +10,9 @@
 namespace kh {
 namespace {
 
-constexpr int kRows = 16, kUnit = 64; // kernels/paged_attention.cu
-constexpr int kMinUnits = 2;          // keys per worker below which more workers cost more than they bring: 128
+constexpr int kRows = 16, kUnit = 64;                  // kernels/paged_attention.cu
+constexpr int kChunkRows = 256, kChunkKeys = 128;      // kernels/paged_attention_chunk.cu
+constexpr int kMinUnits = 2;          // units per worker below which more workers cost more than they bring
 constexpr long kMaxSms = 160;         // workspaces are sized for at most this many SMs
 
 int element_size(int32_t dtype) { return dtype == KH_F32 ? 4 : 2; }
@@ -55,15 +57,27 @@ Shape kernel_shape(int32_t dtype, int32_t head_dim) {
   return s;
 }
 
+// The tensor-memory kernel takes 16-bit types and head sizes of one or two 128-byte swizzle rows, and its copies
+// want boxes of at least eight slots, strides a tensor map can hold, and a scale whose sign keeps maxima maxima.
+bool chunk_kernel_fits(const kh_paged_attention_args &a) {
+  if (a.dtype == KH_F32 || a.head_dim < 64 || a.head_dim > 128 || a.page_size % 8 != 0 || !(a.scale > 0.f)) return false;
+  for (const kh_paged_rows &c : {a.k_cache, a.v_cache})
+    for (const auto &[stride, count] : {std::pair<int64_t, int64_t>{c.page_stride, a.num_pages}, {c.slot_stride, a.page_size}, {c.head_stride, a.k_heads}})
+      if (count > 1 && (stride <= 0 || stride >= (int64_t{1} << 38))) return false;
+  return true;
+}
+// Whether some sequence may have more rows than one tile of the other kernel.
+bool many_rows(const kh_paged_attention_args &a) { return static_cast<int64_t>(a.max_q_len) * (a.q_heads / a.k_heads) > kRows; }
+
 // Grows with `sms` and with every length: the workspace, counted for kMaxSms, covers any device's launch.
-int64_t worker_count(const kh_paged_attention_args &a, const Shape &s, long sms) {
+int64_t worker_count(const kh_paged_attention_args &a, int rows, int unit, int per_sm, long sms) {
   const int64_t group = a.q_heads / a.k_heads;
-  const int64_t items = (a.tokens * group / kRows + a.batch) * a.k_heads; // at most
-  const int64_t units = std::max<int64_t>(1, (static_cast<int64_t>(std::max(a.max_kv_len, 1)) + kUnit - 1) / kUnit);
-  const int64_t most = s.per_sm * std::min(sms, kMaxSms);
+  const int64_t items = (a.tokens * group / rows + a.batch) * a.k_heads; // at most
+  const int64_t units = (static_cast<int64_t>(std::max(a.max_kv_len, 1)) + unit - 1) / unit;
+  const int64_t most = per_sm * std::min(sms, kMaxSms);
   return std::min<int64_t>(most, std::max<int64_t>(1, (items * units + kMinUnits - 1) / kMinUnits));
 }
-int64_t workspace_for(const Shape &s, int64_t workers) { return 2 * workers * kRows * (s.dim * 4 + 8); }
+int64_t workspace_for(int64_t workers, int rows, int dim) { return 2 * workers * rows * (dim * 4 + 8); }
 
 std::string check_stride(const char *name, const void *data, std::initializer_list<std::pair<int64_t, int64_t>> strides, int32_t head_dim,
                          int size, bool output) {
@@ -83,7 +97,11 @@ std::string check_stride(const char *name, const void *data, std::initializer_li
 int64_t paged_attention_workspace(const kh_paged_attention_args &a) {
   if (a.q_heads < 1 || a.k_heads < 1 || a.head_dim < 1 || a.head_dim > 256 || a.tokens < 0 || a.batch < 0) return 0;
   const Shape s = kernel_shape(a.dtype, a.head_dim);
-  return workspace_for(s, worker_count(a, s, kMaxSms));
+  int64_t bytes = workspace_for(worker_count(a, kRows, kUnit, s.per_sm, kMaxSms), kRows, s.dim);
+  // the two kernels run one after the other and use the same memory
+  if (a.dtype != KH_F32 && a.head_dim <= 128 && many_rows(a))
+    bytes = std::max(bytes, workspace_for(worker_count(a, kChunkRows, kChunkKeys, 1, kMaxSms), kChunkRows, s.dim));
+  return bytes;
 }
 
 Result<void> check_paged_attention(const kh_paged_attention_args &a) {
@@ -135,7 +153,6 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
   long sms = query_cu_count(ex.limits());
   if (sms <= 0) sms = 148;
   const Shape s = kernel_shape(a.dtype, a.head_dim);
-  const int64_t workers = worker_count(a, s, sms);
   PagedParams p{};
   const auto stride = [](int64_t v, int64_t count) { return count > 1 ? v : 0; };
   p.q = a.q.data, p.q_token = stride(a.q.token_stride, a.tokens), p.q_head = stride(a.q.head_stride, a.q_heads);
@@ -147,35 +164,85 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
   p.q_start = a.q_start, p.kv_len = a.kv_len;
   p.lse = a.lse;
   p.partial_o = static_cast<float *>(a.workspace);
-  p.partial_ml = static_cast<char *>(a.workspace) + 2 * workers * kRows * s.dim * 4;
   p.status = ex.status_word();
   p.tokens = static_cast<int32_t>(a.tokens), p.batch = a.batch, p.q_heads = a.q_heads, p.k_heads = a.k_heads;
   p.group = a.q_heads / a.k_heads, p.head_dim = a.head_dim;
   p.page_size = a.page_size, p.table_width = a.table_width, p.num_pages = static_cast<int32_t>(a.num_pages);
   p.causal = a.causal, p.window = a.window;
-  p.workers = static_cast<int32_t>(workers), p.min_units = kMinUnits;
-  p.rows_above = 0, p.rows_upto = INT_MAX;
+  p.min_units = kMinUnits;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   const std::string suffix = std::string(a.dtype == KH_F32 ? "f32_" : a.dtype == KH_BF16 ? "bf16_" : "f16_") + std::to_string(s.dim);
-  const auto launch = [&](const std::string &entry, LaunchDims grid, unsigned threads, size_t smem) -> Result<void> {
+  const auto launch = [&](const char *image, const std::string &entry, LaunchDims grid, unsigned threads, size_t smem,
+                          std::initializer_list<TensorMapBytes> maps, int box_rows) -> Result<void> {
     LaunchStep step;
     step.entry = entry;
     step.grid = grid;
     step.block = {threads, 1, 1};
     step.dynamic_smem = smem;
     step.overlap_tail = true;
-    step.param_count = 1;
     LaunchArgs args;
     args.add_struct_bytes(&p, sizeof p);
-    auto fn = ex.function("paged_attention", entry);
+    for (const TensorMapBytes &m : maps) args.add_tensor_map(m);
+    if (box_rows > 0) args.add_scalar<int32_t>(box_rows);
+    step.param_count = static_cast<int>(args.param_count());
+    auto fn = ex.function(image, entry);
     if (!fn) return std::unexpected(fn.error());
     return ex.launch(*fn, step, args, stream);
   };
-  if (auto r = launch("paged_attention_" + suffix, {static_cast<unsigned>(workers), 1, 1}, 32u * s.warps, s.smem); !r) return r;
-  if (workers == 1) return {};
-  // an item is split where a worker's stretch begins inside it: one row of blocks per such place
-  const int64_t rows = std::min<int64_t>(kRows, a.tokens * p.group);
-  return launch("paged_attention_combine_" + suffix, {static_cast<unsigned>(workers - 1), static_cast<unsigned>(rows), 1}, 128, 0);
+  const auto workers = [&](int rows, int unit, int per_sm) {
+    const int64_t n = worker_count(a, rows, unit, per_sm, sms);
+    p.workers = static_cast<int32_t>(n);
+    p.partial_ml = static_cast<char *>(a.workspace) + 2 * n * rows * s.dim * 4;
+    return static_cast<unsigned>(n);
+  };
+  const int64_t all_rows = a.tokens * p.group;
+  p.rows_above = 0, p.rows_upto = INT_MAX;
+
+  if (many_rows(a) && chunk_kernel_fits(a)) {
+    // A sequence of at most 16 rows (a decoding one) goes to the other kernel, unless there can be none: when the
+    // longest length times the batch is no more than the tokens, every sequence has that length.
+    const bool alone = static_cast<int64_t>(a.batch) * a.max_q_len <= a.tokens;
+    if (!alone) p.rows_above = kRows;
+    int box_rows = kChunkKeys; // the largest power of two of slots that divides a page and a tile
+    while (a.page_size % box_rows != 0) box_rows /= 2;
+    TensorMapBytes maps[2];
+    for (int i = 0; i < 2; ++i) {
+      const kh_paged_rows &c = i == 0 ? a.k_cache : a.v_cache;
+      TensorMapSpec t;
+      t.global_address = c.data;
+      t.rank = 4;
+      t.elem_bytes = 2;
+      const int64_t row = a.head_dim; // stands in for the stride of a dimension of size 1
+      const int64_t counts[3] = {a.page_size, a.k_heads, a.num_pages}, strides[3] = {c.slot_stride, c.head_stride, c.page_stride};
+      t.dims[0] = static_cast<uint64_t>(a.head_dim);
+      for (int d = 0; d < 3; ++d) {
+        t.dims[d + 1] = static_cast<uint64_t>(counts[d]);
+        t.strides_bytes[d] = static_cast<uint64_t>(counts[d] > 1 ? strides[d] : row) * 2;
+      }
+      t.box[0] = 64;
+      t.box[1] = static_cast<uint32_t>(box_rows);
+      t.swizzle_bytes = 128;
+      auto map = ex.backend().encode_tensor_map(t);
+      if (!map) return std::unexpected(map.error());
+      maps[i] = *map;
+    }
+    const unsigned n = workers(kChunkRows, kChunkKeys, 1);
+    const int stages = s.dim == 128 ? 5 : 8;
+    const size_t smem = static_cast<size_t>(2 + stages) * kChunkKeys * s.dim * 2 + 1024;
+    if (auto r = launch("paged_attention_chunk", "paged_attention_chunk_" + suffix, {n, 1, 1}, 512, smem, {maps[0], maps[1]}, box_rows); !r) return r;
+    if (n > 1) {
+      // an item is split where a worker's stretch begins inside it: 32 rows of it per block
+      const unsigned y = static_cast<unsigned>((std::min<int64_t>(kChunkRows, all_rows) + 31) / 32);
+      if (auto r = launch("paged_attention_chunk", "paged_attention_chunk_combine_" + suffix, {n - 1, y, 1}, 128, 0, {}, 0); !r) return r;
+    }
+    if (alone) return {};
+    p.rows_above = 0, p.rows_upto = kRows;
+  }
+  const unsigned n = workers(kRows, kUnit, s.per_sm);
+  if (auto r = launch("paged_attention", "paged_attention_" + suffix, {n, 1, 1}, 32u * s.warps, s.smem, {}, 0); !r) return r;
+  if (n == 1) return {};
+  const unsigned y = static_cast<unsigned>(std::min<int64_t>(kRows, all_rows)); // a row per block
+  return launch("paged_attention", "paged_attention_combine_" + suffix, {n - 1, y, 1}, 128, 0, {}, 0);
 }
 
 } // namespace kh
