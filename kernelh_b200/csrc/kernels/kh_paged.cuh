@@ -8,11 +8,12 @@
 //
 // Work. An item is (sequence, key/value head, row block) and takes n units of kUnit keys, n the same for all
 // items of a sequence (its whole key range; the causal mask cuts the units at an item's end, which cost
-// nothing). All units of all items form one line, and every worker (a block) takes an equal stretch of it,
-// whatever the lengths are: a worker finishes the item it starts in, does whole ones, and leaves the last one
+// nothing), and kPad more that stand for its start and end. All of these of all items form one line, and every
+// worker (a block) takes an equal stretch of it, whatever the lengths are: a worker finishes the item it starts in, does whole ones, and leaves the last one
 // to the next worker. Items that more than one worker touches leave (max, sum, unnormalised row) in the
-// workspace: slot 2w + 1 for the worker that starts an item, 2w for those that continue it; a second launch
-// adds them up in the order of the keys. The line is laid out from q_start and kv_len on the device, so a
+// workspace: slot 2w + 1 for the worker that starts an item, 2w for those that continue it. The first worker
+// that begins inside an item also leaves a note of it, and a second launch adds the parts up in the order of
+// the keys. The line is laid out from q_start and kv_len on the device, so a
 // captured call follows lengths that change between replays.
 #pragma once
 
@@ -36,6 +37,7 @@ struct PagedParams {
   float *lse;       // [tokens, q_heads] or nullptr
   float *partial_o; // [2 * workers][rows of a block][padded head_dim]
   float2 *partial_ml;
+  struct SplitItem *split_items; // [workers]
   uint32_t *status;
   int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, table_width, num_pages;
   int32_t causal, window;  // window 0: none
@@ -44,13 +46,18 @@ struct PagedParams {
   float scale_log2;              // scale * log2(e): scores are kept in exp2 units
 };
 
+// How a kernel cuts its work (kRows, kUnit) and what an item costs beside its units (kPad, in units).
+template <int kRows_, int kUnit_, int kPad_> struct Grain {
+  static constexpr int kRows = kRows_, kUnit = kUnit_, kPad = kPad_;
+};
 struct Sequence {
   int q0, tokens, rows, kv; // first token, new tokens, tokens * group, keys
   int blocks, first_unit, units; // row blocks; the key units that any row sees
+  int span;                      // an item's length on the line
 };
 
 // The sequence's shape, with every offset forced into range (and reported when it was not).
-template <int kRows, int kUnit> __device__ __forceinline__ Sequence sequence(const PagedParams &P, int b) {
+template <typename G> __device__ __forceinline__ Sequence sequence(const PagedParams &P, int b) {
   Sequence s;
   s.q0 = P.q_start[b];
   const int q1 = P.q_start[b + 1];
@@ -66,15 +73,16 @@ template <int kRows, int kUnit> __device__ __forceinline__ Sequence sequence(con
   }
   const int64_t rows = static_cast<int64_t>(s.tokens) * P.group;
   s.rows = rows > P.rows_above && rows <= P.rows_upto ? static_cast<int>(rows) : 0;
-  s.blocks = (s.rows + kRows - 1) / kRows;
+  s.blocks = (s.rows + G::kRows - 1) / G::kRows;
   const int64_t first = P.window > 0 ? static_cast<int64_t>(s.kv) - s.tokens - P.window + 1 : 0;
-  s.first_unit = first > 0 ? static_cast<int>(first / kUnit) : 0;
-  s.units = max(1, (s.kv + kUnit - 1) / kUnit - s.first_unit); // an item without keys still has its zeros to write
+  s.first_unit = first > 0 ? static_cast<int>(first / G::kUnit) : 0;
+  s.units = max(1, (s.kv + G::kUnit - 1) / G::kUnit - s.first_unit); // an item without keys still has its zeros to write
+  s.span = s.units + G::kPad;
   return s;
 }
-template <int kRows, int kUnit> __device__ __forceinline__ int64_t sequence_units(const PagedParams &P, int b) {
-  const Sequence s = sequence<kRows, kUnit>(P, b);
-  return static_cast<int64_t>(s.blocks) * s.units * P.k_heads;
+template <typename G> __device__ __forceinline__ int64_t sequence_span(const PagedParams &P, int b) {
+  const Sequence s = sequence<G>(P, b);
+  return static_cast<int64_t>(s.blocks) * s.span * P.k_heads;
 }
 
 // Row blocks are walked from both ends (0, last, 1, last - 1, ...): under the causal mask the work of two
@@ -113,10 +121,10 @@ template <int kThreads> __device__ __forceinline__ int64_t block_scan(int64_t v,
   return all;
 }
 
-template <int kThreads, int kRows, int kUnit>
+template <int kThreads, typename G>
 __device__ __forceinline__ Line measure_line(const PagedParams &P, LineScratch<kThreads> &s) {
   int64_t mine = 0, inclusive;
-  for (int b = threadIdx.x; b < P.batch; b += kThreads) mine += sequence_units<kRows, kUnit>(P, b);
+  for (int b = threadIdx.x; b < P.batch; b += kThreads) mine += sequence_span<G>(P, b);
   Line line;
   line.total = block_scan<kThreads>(mine, inclusive, s.warp_sum);
   const int64_t most = (line.total + P.min_units - 1) / P.min_units;
@@ -128,12 +136,12 @@ __device__ __forceinline__ int64_t stretch(const Line &line, int w) {
   return line.total / line.workers * w + line.total % line.workers * w / line.workers;
 }
 // The sequence that unit `at` (< total) belongs to, and where that sequence starts on the line.
-template <int kThreads, int kRows, int kUnit>
+template <int kThreads, typename G>
 __device__ __forceinline__ void locate(const PagedParams &P, int64_t at, LineScratch<kThreads> &s, int &b_out, int64_t &start) {
   int64_t before = 0;
   for (int base = 0; base < P.batch; base += kThreads) {
     const int b = base + static_cast<int>(threadIdx.x);
-    const int64_t mine = b < P.batch ? sequence_units<kRows, kUnit>(P, b) : 0;
+    const int64_t mine = b < P.batch ? sequence_span<G>(P, b) : 0;
     int64_t inclusive;
     const int64_t all = block_scan<kThreads>(mine, inclusive, s.warp_sum);
     if (at < before + all) {
@@ -151,58 +159,55 @@ __device__ __forceinline__ void locate(const PagedParams &P, int64_t at, LineScr
   __syncthreads();
 }
 
-// The item that worker w's stretch (w > 0) begins inside of, if no earlier stretch does, and its parts:
-// part 0 in slot 2 (w - 1) + 1, part p in slot 2 (w - 1 + p).
-struct Split {
-  Sequence s;
-  int h, row0, w, parts; // parts 0: nothing to add up here
-  __device__ __forceinline__ int64_t slot(int p) const { return 2 * static_cast<int64_t>(w - 1 + p) + (p == 0 ? 1 : 0); }
+// The item that worker w's stretch begins inside of, if no earlier stretch does (parts 0 otherwise). Its part 0
+// lies in slot 2 (w - 1) + 1, part p in slot 2 (w - 1 + p).
+struct alignas(32) SplitItem {
+  int32_t q0, row0, rows, h, parts; // rows: of the item
 };
-template <int kThreads, int kRows, int kUnit> __device__ __forceinline__ Split find_split(const PagedParams &P, LineScratch<kThreads> &scratch) {
-  Split x{};
-  const Line line = measure_line<kThreads, kRows, kUnit>(P, scratch);
-  x.w = blockIdx.x + 1;
-  if (x.w >= line.workers) return x;
-  const int64_t at = stretch(line, x.w);
-  int b;
-  int64_t start;
-  locate<kThreads, kRows, kUnit>(P, at, scratch, b, start);
-  x.s = sequence<kRows, kUnit>(P, b);
-  const int64_t item = (at - start) / x.s.units; // head * blocks + place of the row block
-  const int64_t begin = start + item * x.s.units, end = begin + x.s.units;
-  if (begin == at || begin < stretch(line, x.w - 1)) return x; // nothing split here, or an earlier block's
-  x.h = static_cast<int>(item / x.s.blocks);
-  x.row0 = block_of(static_cast<int>(item - static_cast<int64_t>(x.h) * x.s.blocks), x.s.blocks) * kRows;
-  int last = x.w; // the last worker with a part
-  while (last + 1 < line.workers && stretch(line, last + 1) < end) ++last;
-  x.parts = last - x.w + 2;
-  return x;
+__device__ __forceinline__ int64_t part_slot(int w, int p) { return 2 * static_cast<int64_t>(w - 1 + p) + (p == 0 ? 1 : 0); }
+// One thread of worker w notes it down. `at`: where the stretch begins, in sequence b, which begins at `start`.
+template <typename G>
+__device__ __forceinline__ void note_split(const PagedParams &P, const Line &line, int w, int64_t at, int b, int64_t start) {
+  SplitItem x{};
+  if (w > 0 && w < line.workers) {
+    const Sequence s = sequence<G>(P, b);
+    const int64_t item = (at - start) / s.span; // head * blocks + place of the row block
+    const int64_t begin = start + item * s.span, end = begin + s.units;
+    if (begin < at && at < end && begin >= stretch(line, w - 1)) {
+      x.q0 = s.q0;
+      x.h = static_cast<int>(item / s.blocks);
+      x.row0 = block_of(static_cast<int>(item - static_cast<int64_t>(x.h) * s.blocks), s.blocks) * G::kRows;
+      x.rows = min(G::kRows, s.rows - x.row0);
+      int last = w; // the last worker with a part
+      while (last + 1 < line.workers && stretch(line, last + 1) < end) ++last;
+      x.parts = last - w + 2;
+    }
+  }
+  P.split_items[w] = x;
 }
 
 // Adds up the parts of one row, for items with few rows and many parts: block (w - 1, y) takes row y of w's
 // item. Its warps take every kThreads / 32-th part each with a running maximum and are added up in order.
-template <typename T, int kThreads, int kRows, int kUnit, int kDim, typename Store>
-__device__ __forceinline__ void combine_body(const PagedParams &P, Store store) {
-  __shared__ LineScratch<kThreads> scratch;
+template <int kThreads, int kRows, int kDim, typename Store> __device__ __forceinline__ void combine_row(const PagedParams &P, Store store) {
   __shared__ float s_row[kThreads / 32][kDim];
   __shared__ float2 s_ml[kThreads / 32];
   khd::grid_dependency_wait();
-  const Split x = find_split<kThreads, kRows, kUnit>(P, scratch);
-  const Sequence &s = x.s;
-  const int row = x.row0 + static_cast<int>(blockIdx.y), h = x.h, parts = x.parts;
-  if (parts == 0 || static_cast<int>(blockIdx.y) >= kRows || row >= s.rows) return;
+  const int w = blockIdx.x + 1;
+  const SplitItem x = P.split_items[w];
+  const int in_block = static_cast<int>(blockIdx.y), row = x.row0 + in_block;
+  if (x.parts == 0 || in_block >= x.rows) return;
   constexpr int kWarps = kThreads / 32, kPer = kDim / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float m = -INFINITY, l = 0.f, acc[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  for (int p = warp; p < parts; p += kWarps) {
-    const int64_t slot = x.slot(p);
-    const float2 ml = P.partial_ml[slot * kRows + blockIdx.y];
-    const float *src = P.partial_o + (slot * kRows + blockIdx.y) * kDim + lane * kPer;
+#pragma unroll 4
+  for (int p = warp; p < x.parts; p += kWarps) {
+    const int64_t at = part_slot(w, p) * kRows + in_block;
+    const float2 ml = P.partial_ml[at];
     float y[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) y[i] = src[i];
+    for (int i = 0; i < kPer; ++i) y[i] = P.partial_o[at * kDim + i * 32 + lane];
     const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
     const float f_old = exp2f(m - ref), f_new = exp2f(ml.x - ref);
     l = l * f_old + ml.y * f_new;
@@ -211,7 +216,7 @@ __device__ __forceinline__ void combine_body(const PagedParams &P, Store store) 
     m = m_new;
   }
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) s_row[warp][lane * kPer + i] = acc[i];
+  for (int i = 0; i < kPer; ++i) s_row[warp][i * 32 + lane] = acc[i];
   if (lane == 0) s_ml[warp] = make_float2(m, l);
   __syncthreads();
   float top = -INFINITY;
@@ -224,7 +229,7 @@ __device__ __forceinline__ void combine_body(const PagedParams &P, Store store) 
     f[i] = exp2f(s_ml[i].x - ref);
     sum += s_ml[i].y * f[i];
   }
-  const int token = s.q0 + row / P.group, head = h * P.group + row % P.group;
+  const int token = x.q0 + row / P.group, head = x.h * P.group + row % P.group;
   for (int c = threadIdx.x; c < P.head_dim; c += kThreads) {
     float v = 0.f;
 #pragma unroll
@@ -235,41 +240,66 @@ __device__ __forceinline__ void combine_body(const PagedParams &P, Store store) 
     P.lse[static_cast<int64_t>(token) * P.q_heads + head] = sum != 0.f ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
 }
 
-// The same for items with many rows, which have few parts: block (w - 1, y) takes the rows y * 32 .. + 31 of w's
-// item, a warp takes whole rows and goes through their parts in order.
-template <int kThreads, int kRows, int kUnit, int kDim, typename Store>
-__device__ __forceinline__ void combine_rows(const PagedParams &P, Store store) {
-  __shared__ LineScratch<kThreads> scratch;
+// The same for items with many rows, which have few parts: block (w - 1, y) takes the rows y * kBlockRows .. of w's
+// item, a warp two of them at once, a row's parts in order.
+constexpr int kBlockRows = 16;
+template <int kRows, int kDim, typename Store> __device__ __forceinline__ void combine_rows(const PagedParams &P, Store store) {
   khd::grid_dependency_wait();
-  const Split x = find_split<kThreads, kRows, kUnit>(P, scratch);
-  if (x.parts == 0) return;
-  constexpr int kPer = kDim / 32, kWarps = kThreads / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = warp; i < 32; i += kWarps) {
-    const int in_block = static_cast<int>(blockIdx.y) * 32 + i, row = x.row0 + in_block;
-    if (in_block >= kRows || row >= x.s.rows) return;
-    float m = -INFINITY, l = 0.f, acc[kPer];
+  const int w = blockIdx.x + 1;
+  const SplitItem x = P.split_items[w];
+  constexpr int kPer = kDim / 32, kAtOnce = kBlockRows / 8;
+  const int lane = threadIdx.x & 31, first = static_cast<int>(blockIdx.y) * kBlockRows + static_cast<int>(threadIdx.x >> 5) * kAtOnce;
+  if (x.parts == 0 || first >= x.rows) return;
+  float m[kAtOnce], l[kAtOnce], acc[kAtOnce][kPer];
 #pragma unroll
-    for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
-    for (int p = 0; p < x.parts; ++p) {
-      const int64_t at = x.slot(p) * kRows + in_block;
-      const float2 ml = P.partial_ml[at];
-      float y[kPer];
+  for (int i = 0; i < kAtOnce; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) y[c] = P.partial_o[at * kDim + c * 32 + lane];
-      const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
-      const float f_old = exp2f(m - ref), f_new = exp2f(ml.x - ref);
-      l = l * f_old + ml.y * f_new;
+    for (int c = 0; c < kPer; ++c) acc[i][c] = 0.f;
+  }
+  float2 ml[kAtOnce];
+  float y[kAtOnce][kPer];
+  const auto fetch = [&](int p) {
+    const int64_t slot = part_slot(w, p) * kRows;
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) acc[c] = acc[c] * f_old + y[c] * f_new;
-      m = m_new;
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t at = slot + min(first + i, x.rows - 1);
+      ml[i] = P.partial_ml[at];
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) y[i][c] = P.partial_o[at * kDim + c * 32 + lane];
     }
-    const int token = x.s.q0 + row / P.group, head = x.h * P.group + row % P.group;
+  };
+  fetch(0);
+  for (int p = 0; p < x.parts; ++p) {
+    float2 ml0[kAtOnce];
+    float y0[kAtOnce][kPer];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      ml0[i] = ml[i];
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) y0[i][c] = y[i][c];
+    }
+    if (p + 1 < x.parts) fetch(p + 1); // the next part is on its way while this one is added
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float m_new = fmaxf(m[i], ml0[i].x), ref = m_new == -INFINITY ? 0.f : m_new;
+      const float f_old = exp2f(m[i] - ref), f_new = exp2f(ml0[i].x - ref);
+      l[i] = l[i] * f_old + ml0[i].y * f_new;
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) acc[i][c] = acc[i][c] * f_old + y0[i][c] * f_new;
+      m[i] = m_new;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) {
+    if (first + i >= x.rows) return;
+    const int row = x.row0 + first + i, token = x.q0 + row / P.group, head = x.h * P.group + row % P.group;
 #pragma unroll
     for (int c = 0; c < kPer; ++c)
-      if (c * 32 + lane < P.head_dim) store(token, head, c * 32 + lane, l != 0.f ? acc[c] / l : 0.f);
+      if (c * 32 + lane < P.head_dim) store(token, head, c * 32 + lane, l[i] != 0.f ? acc[i][c] / l[i] : 0.f);
     if (lane == 0 && P.lse != nullptr)
-      P.lse[static_cast<int64_t>(token) * P.q_heads + head] = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+      P.lse[static_cast<int64_t>(token) * P.q_heads + head] = l[i] != 0.f ? (m[i] + log2f(l[i])) * 0.69314718055994531f : -INFINITY;
   }
 }
 

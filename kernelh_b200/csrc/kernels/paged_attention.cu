@@ -32,6 +32,7 @@ template <typename T, int kDim> struct Config {
   static constexpr int kWarps = kRowBytes <= 512 ? 4 : 2; // 3 stages of 16 keys and values per warp must fit
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kUnit = 64; // keys of a unit: the same for every type, so that the host can count
+  using Cut = khp::Grain<kRows, kUnit, 1>; // an item's start and end cost about a unit
   static constexpr int kSteps = kUnit / (kKeys * kWarps);
   static constexpr int kPitch = kRowBytes + 16; // bytes between rows: ldmatrix and fp32 reads without bank conflicts
   static constexpr int kTile = kKeys * kPitch;
@@ -195,6 +196,7 @@ __device__ __forceinline__ void value_tile(const float (&p)[2][4], uint32_t tile
 
 template <typename T, int kDim> __device__ __forceinline__ void attention_body(const PagedParams &P) {
   using Cfg = Config<T, kDim>;
+  using Cut = typename Cfg::Cut;
   constexpr int kThreads = Cfg::kThreads, kWarps = Cfg::kWarps, kUnit = Cfg::kUnit;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ khp::LineScratch<kThreads> scratch;
@@ -207,30 +209,38 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
   }
   khd::grid_dependency_wait();
   khd::grid_dependents_may_launch();
-  const khp::Line line = khp::measure_line<kThreads, kRows, kUnit>(P, scratch);
+  const khp::Line line = khp::measure_line<kThreads, Cut>(P, scratch);
   const int w = blockIdx.x;
-  if (w >= line.workers) return;
+  if (w >= line.workers) {
+    if (threadIdx.x == 0) P.split_items[w] = khp::SplitItem{};
+    return;
+  }
   int64_t at = khp::stretch(line, w);
   const int64_t until = khp::stretch(line, w + 1);
   const int64_t from = at;
   int b;
   int64_t start;
-  khp::locate<kThreads, kRows, kUnit>(P, at, scratch, b, start);
-  khp::Sequence s = khp::sequence<kRows, kUnit>(P, b);
+  khp::locate<kThreads, Cut>(P, at, scratch, b, start);
+  if (threadIdx.x == 0) khp::note_split<Cut>(P, line, w, at, b, start);
+  khp::Sequence s = khp::sequence<Cut>(P, b);
 
   const int chunks_per_row = P.head_dim * static_cast<int>(sizeof(T)) / 16; // 16-byte pieces that exist
   while (at < until) {
-    int64_t size = static_cast<int64_t>(s.blocks) * s.units * P.k_heads;
+    int64_t size = static_cast<int64_t>(s.blocks) * s.span * P.k_heads;
     while (at >= start + size) { // on to the next sequence that has rows
       start += size;
-      s = khp::sequence<kRows, kUnit>(P, ++b);
-      size = static_cast<int64_t>(s.blocks) * s.units * P.k_heads;
+      s = khp::sequence<Cut>(P, ++b);
+      size = static_cast<int64_t>(s.blocks) * s.span * P.k_heads;
     }
-    const int64_t item = (at - start) / s.units;
-    const int64_t begin = start + item * s.units, end = begin + s.units;
+    const int64_t item = (at - start) / s.span;
+    const int64_t begin = start + item * s.span, end = begin + s.span;
+    if (at - begin >= s.units) { // what is left of the item is only what stands for its end
+      at = end;
+      continue;
+    }
     const int h = static_cast<int>(item / s.blocks);
     const int block = khp::block_of(static_cast<int>(item - static_cast<int64_t>(h) * s.blocks), s.blocks);
-    const int unit0 = static_cast<int>(at - begin), unit1 = static_cast<int>((until < end ? until : end) - begin);
+    const int unit0 = static_cast<int>(at - begin), unit1 = static_cast<int>(min((until < end ? until : end) - begin, static_cast<int64_t>(s.units)));
     const int row0 = block * kRows, rows_here = min(kRows, s.rows - row0);
     // keys that rows of this block see, and the part of them in this stretch
     const int t_first = row0 / P.group, t_last = (row0 + rows_here - 1) / P.group;
@@ -417,12 +427,12 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
       for (int i = threadIdx.x * 16; i < Cfg::kSmem; i += kThreads * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
       __syncthreads();
     }
-    at = begin + unit1;
+    at = until < end ? until : end;
   }
 }
 
 template <typename T, int kDim> __device__ __forceinline__ void combine(const PagedParams &P) {
-  khp::combine_body<T, 128, kRows, Config<T, kDim>::kUnit, kDim>(P, [&](int token, int head, int c, float v) {
+  khp::combine_row<128, kRows, kDim>(P, [&](int token, int head, int c, float v) {
     reinterpret_cast<T *>(P.o)[token * P.o_token + head * P.o_head + c] = from_float<T>(v);
   });
 }

@@ -9,7 +9,8 @@
 //
 // One block per SM, 16 warps. Warpgroups 0 and 1, a thread per row, are the softmax of the two tiles; while one
 // works, the tensor core does the other tile's P V and the next Q K^T, so the two keep it busy in turns. Warp 8
-// issues the matrix instructions, warp 9 the copies: the boxes of a tile are looked up in the page table by one
+// issues the matrix instructions, warp 10 the copies, warps 12 to 15 bring in the queries of the next item while this
+// one's last tile is worked on. The boxes of a tile of keys are looked up in the page table by one
 // lane each and fetched by TMA straight out of the pages (a box is the largest power of two of slots that divides
 // the page, so none crosses a page), keys and values through one ring. Pages therefore cost nothing but the
 // look-up.
@@ -23,7 +24,12 @@
 // item that have any.
 //
 // Tensor-bound: 4 * 128 values * 256 rows * 128 keys = 16.8 Mflop per tile pair, 2048 clocks at the dense
-// 16-bit rate; the 32768 exponentials of a pair take the special-function units the same 2048 clocks.
+// 16-bit rate; the 32768 exponentials of a pair take the special-function units the same 2048 clocks. Measured (a
+// 2048-token chunk after 14336 tokens, 32 heads over 8, bf16): 441 us = 1.17 PFLOP/s, 2000 ns a pair; without the
+// exponentials 400, without any softmax 365 (the products of a tile follow one another through four barriers).
+// Measured and dropped: P handed over in two (447) or four (549) parts, an issuing warp per tile (445), 2 or 3 of 8
+// exponentials by a polynomial on the multiply-add pipes (469, 490), two threads per row (556), the row maximum as a
+// thread's first score (no change: 490 against 487 at the time).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -37,9 +43,10 @@ using khp::PagedParams;
 constexpr int kTileRows = 128;
 constexpr int kRows = 2 * kTileRows; // rows of an item
 constexpr int kKeys = 128;           // keys of a tile
+using Cut = khp::Grain<kRows, kKeys, 3>; // an item's queries, first scores and output cost about three tiles
 constexpr int kThreads = 512;
 constexpr int kMaxStages = 8;
-constexpr int kIssueWarp = 8, kLoadWarp = 9;
+constexpr int kIssueWarp = 8, kLoadWarp = 10, kQueryWarp = 12, kQueryWarps = 4;
 // registers after the warpgroups have traded them: two softmax groups, control, idle; 4 x 128 at launch
 constexpr int kRegsSoftmax = 200, kRegsControl = 56;
 constexpr float kLazy = 8.f;
@@ -79,6 +86,19 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t addr, const uint32_t (&r)
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// The largest of three; NaN if any is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// One arrival for the warp, after all its lanes (an arrival of every thread costs the barrier a turn each).
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) khd::mbar_arrive(bar);
+}
 
 // Operand descriptor of an MN-major tile in the 128-byte swizzle: rows (along K: keys) of 128 bytes hold 64
 // values along MN; 8 rows are 1024 bytes, the next 64 values along MN lie `half_bytes` on. Fields as in
@@ -124,20 +144,25 @@ struct Walker {
   int64_t at, until, from, start;
   int b, w;
   __device__ __forceinline__ bool next(const PagedParams &P, Work &k) {
-    if (at >= until) return false;
-    k.s = khp::sequence<kRows, kKeys>(P, b);
-    int64_t size = static_cast<int64_t>(k.s.blocks) * k.s.units * P.k_heads;
-    while (at >= start + size) {
-      start += size;
-      k.s = khp::sequence<kRows, kKeys>(P, ++b);
-      size = static_cast<int64_t>(k.s.blocks) * k.s.units * P.k_heads;
+    int64_t item, begin, end;
+    for (;;) {
+      if (at >= until) return false;
+      k.s = khp::sequence<Cut>(P, b);
+      int64_t size = static_cast<int64_t>(k.s.blocks) * k.s.span * P.k_heads;
+      while (at >= start + size) {
+        start += size;
+        k.s = khp::sequence<Cut>(P, ++b);
+        size = static_cast<int64_t>(k.s.blocks) * k.s.span * P.k_heads;
+      }
+      item = (at - start) / k.s.span;
+      begin = start + item * k.s.span, end = begin + k.s.span;
+      if (at - begin < k.s.units) break;
+      at = end; // what is left of the item is only what stands for its end
     }
-    const int64_t item = (at - start) / k.s.units;
-    const int64_t begin = start + item * k.s.units, end = begin + k.s.units;
     k.b = b;
     k.h = static_cast<int>(item / k.s.blocks);
     const int block = khp::block_of(static_cast<int>(item - static_cast<int64_t>(k.h) * k.s.blocks), k.s.blocks);
-    const int unit0 = static_cast<int>(at - begin), unit1 = static_cast<int>((until < end ? until : end) - begin);
+    const int unit0 = static_cast<int>(at - begin), unit1 = static_cast<int>(min((until < end ? until : end) - begin, static_cast<int64_t>(k.s.units)));
     k.row0 = block * kRows;
     k.rows = min(kRows, k.s.rows - k.row0);
     const int t_first = k.row0 / P.group, t_last = (k.row0 + k.rows - 1) / P.group;
@@ -149,7 +174,7 @@ struct Walker {
     k.key_b = static_cast<int>(min(static_cast<int64_t>(k.s.first_unit + unit1) * kKeys, static_cast<int64_t>(hi)));
     k.tiles = k.key_b > k.key_a ? (k.key_b - k.key_a + kKeys - 1) / kKeys : 0;
     k.part = unit0 == 0 && unit1 == k.s.units ? -1 : (begin < from ? 2 * static_cast<int64_t>(w) : 2 * static_cast<int64_t>(w) + 1);
-    at = begin + unit1;
+    at = until < end ? until : end;
     return true;
   }
 };
@@ -161,7 +186,7 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
   constexpr uint32_t kHalfBytes = kKeys * 128; // 128 rows of 128 bytes
   constexpr int kStages = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[8 + 2 * kMaxStages];
+  __shared__ __align__(8) uint64_t bars[10 + 2 * kMaxStages];
   __shared__ khp::LineScratch<kThreads> scratch;
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
@@ -170,14 +195,16 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
   const uint32_t smem_q = (khd::smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t smem_ring = smem_q + 2 * Cfg::kTileBytes;
   const uint32_t bar_q = khd::smem_u32(&bars[0]), bar_s = khd::smem_u32(&bars[2]), bar_p = khd::smem_u32(&bars[4]),
-                 bar_o = khd::smem_u32(&bars[6]), bar_full = khd::smem_u32(&bars[8]), bar_empty = khd::smem_u32(&bars[8 + kMaxStages]);
+                 bar_o = khd::smem_u32(&bars[6]), bar_q_free = khd::smem_u32(&bars[8]), bar_full = khd::smem_u32(&bars[10]),
+                 bar_empty = khd::smem_u32(&bars[10 + kMaxStages]);
   if (threadIdx.x == 0) {
     s_abort = 0;
     for (int g = 0; g < 2; ++g) {
-      khd::mbar_init(bar_q + 8 * g, kTileRows); // Q_g is in shared memory
-      khd::mbar_init(bar_s + 8 * g, 1);         // S_g is done (and every product before it)
-      khd::mbar_init(bar_p + 8 * g, kTileRows); // P_g is in tensor memory
-      khd::mbar_init(bar_o + 8 * g, 1);         // O_g is complete
+      khd::mbar_init(bar_q + 8 * g, kQueryWarps); // Q_g is in shared memory
+      khd::mbar_init(bar_q_free + 8 * g, 1);           // the last S_g of an item is done: Q_g may go
+      khd::mbar_init(bar_s + 8 * g, 1);                // S_g is done (and every product before it)
+      khd::mbar_init(bar_p + 8 * g, 4);           // P_g is in tensor memory (an arrival per warp)
+      khd::mbar_init(bar_o + 8 * g, 1);                // O_g is complete
     }
     for (int i = 0; i < kStages; ++i) {
       khd::mbar_init(bar_full + 8 * i, 1);
@@ -198,14 +225,15 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
   khd::grid_dependency_wait();
   khd::grid_dependents_may_launch();
 
-  const khp::Line line = khp::measure_line<kThreads, kRows, kKeys>(P, scratch);
+  const khp::Line line = khp::measure_line<kThreads, Cut>(P, scratch);
   Walker walker{};
   walker.w = blockIdx.x;
   if (static_cast<int>(blockIdx.x) < line.workers) {
     walker.from = walker.at = khp::stretch(line, walker.w);
     walker.until = khp::stretch(line, walker.w + 1);
-    khp::locate<kThreads, kRows, kKeys>(P, walker.at, scratch, walker.b, walker.start);
+    khp::locate<kThreads, Cut>(P, walker.at, scratch, walker.b, walker.start);
   }
+  if (threadIdx.x == kThreads - 1) khp::note_split<Cut>(P, line, walker.w, walker.at, walker.b, walker.start);
   Work k;
 
   if (warp >= 8) {
@@ -250,7 +278,9 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
         }
       }
     } else if (warp == kIssueWarp) {
-      // ---- matrix instructions, issued by one lane; the warp walks the loop together -------------------------
+      // ---- matrix instructions, issued by one lane; the warp walks the loop together. Everything the instructions take
+      //      is worked out warp-uniformly, outside the elected lane's branch: lengths come from lane 0 by shuffle,
+      //      descriptors are a base plus constants (the address field counts 16 bytes). ----------------------------
       const bool leader = khd::elect_one();
       constexpr uint32_t kTypes = (Types<T>::kFormat << 7) | (Types<T>::kFormat << 10);
       constexpr uint32_t idesc_s = khd::umma_idesc_f16(kTileRows, kKeys) | kTypes;
@@ -259,9 +289,7 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
       bool ok = true;
       const auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code, uint32_t detail) {
         const bool ready = khd::mbar_wait(bar, parity, &s_abort, P.status, code, detail);
-        if (!__all_sync(0xffffffffu, ready)) return false;
-        khd::tc_fence_after_sync();
-        return true;
+        return __all_sync(0xffffffffu, ready) != 0;
       };
       const auto advance = [&] {
         if (++slot == kStages) {
@@ -269,73 +297,109 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
           phase ^= 1u;
         }
       };
-      const auto issue_s = [&](int g, uint32_t tile) {
+      const uint64_t desc_q = khd::umma_desc_k128(smem_q);
+      const uint64_t desc_k = khd::umma_desc_k128(smem_ring), desc_v = umma_desc_mn128(smem_ring, kHalfBytes);
+      constexpr uint32_t kStep = Cfg::kTileBytes >> 4;
+      const auto issue_s = [&](int g, uint32_t k_slot, bool last, bool done) {
+        const uint64_t a = desc_q + static_cast<uint32_t>(g) * kStep, b = desc_k + k_slot * kStep;
         if (leader) {
 #pragma unroll
           for (int i = 0; i < kDim / 16; ++i) {
-            const uint32_t off = (i >> 2) * kHalfBytes + (i & 3) * 32;
-            khd::umma_f16_ss(tmem + g * 128, khd::umma_desc_k128(smem_q + g * Cfg::kTileBytes + off), khd::umma_desc_k128(tile + off), idesc_s,
-                             i != 0);
+            const uint32_t off = (i >> 2) * (kHalfBytes >> 4) + (i & 3) * 2;
+            khd::umma_f16_ss(tmem + g * 128, a + off, b + off, idesc_s, i != 0);
           }
           khd::umma_commit(bar_s + 8 * g);
+          if (done) khd::umma_commit(bar_empty + 8 * k_slot);
+          if (last) khd::umma_commit(bar_q_free + 8 * g);
         }
         __syncwarp();
       };
-      while (ok && walker.next(P, k)) {
-        if (k.tiles == 0) continue;
-        const int groups = k.rows > kTileRows ? 2 : 1;
+      while (ok && __any_sync(0xffffffffu, walker.next(P, k))) {
+        const int tiles = __shfl_sync(0xffffffffu, k.tiles, 0), groups = __shfl_sync(0xffffffffu, k.rows, 0) > kTileRows ? 2 : 1;
+        const int key_a = __shfl_sync(0xffffffffu, k.key_a, 0), key_b = __shfl_sync(0xffffffffu, k.key_b, 0),
+                  key_lo = __shfl_sync(0xffffffffu, k.key_lo, 0);
+        if (tiles == 0) continue;
         for (int g = 0; g < groups && ok; ++g) {
           ok = wait(bar_q + 8 * g, q_phase[g], khd::kStatusEpilogueWaitTimeout, 6100u);
           q_phase[g] ^= 1u;
         }
         ok = ok && wait(bar_full + 8 * slot, phase, khd::kStatusTmaWaitTimeout, 6200u);
         if (!ok) break;
-        for (int g = 0; g < groups; ++g) issue_s(g, smem_ring + slot * Cfg::kTileBytes);
-        if (leader) khd::umma_commit(bar_empty + 8 * slot);
-        __syncwarp();
+        khd::tc_fence_after_sync();
+        for (int g = 0; g < groups; ++g) issue_s(g, slot, tiles == 1, g == groups - 1);
         advance();
-        for (int j = 0; j < k.tiles && ok; ++j) {
-          const uint32_t v_slot = slot, v_tile = smem_ring + slot * Cfg::kTileBytes;
+        for (int j = 0; j < tiles && ok; ++j) {
+          const uint32_t v_slot = slot;
+          const uint64_t v = desc_v + v_slot * kStep;
           ok = wait(bar_full + 8 * slot, phase, khd::kStatusTmaWaitTimeout, 6300u);
           if (!ok) break;
           advance();
           // rows of V that no query sees: zeros
-          const int key0 = k.key_a + j * kKeys, lo = max(0, k.key_lo - key0), hi = min(kKeys, k.key_b - key0);
+          const int key0 = key_a + j * kKeys, lo = max(0, key_lo - key0), hi = min(kKeys, key_b - key0);
           if (lo > 0 || hi < kKeys) {
             for (int i = lane; i < kHalves * kKeys * 8; i += 32) {
               const int row = (i >> 3) & (kKeys - 1);
               if (row < lo || row >= hi)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_tile + (i >> 10) * kHalfBytes + (i & 1023) * 16), "r"(0) : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem_ring + v_slot * Cfg::kTileBytes + (i >> 10) * kHalfBytes +
+                                                                                  (i & 1023) * 16),
+                             "r"(0)
+                             : "memory");
             }
             fence_async_shared();
             __syncwarp();
           }
-          const bool more = j + 1 < k.tiles;
-          for (int g = 0; g < groups && ok; ++g) {
-            ok = wait(bar_p + 8 * g, p_phase[g], khd::kStatusEpilogueWaitTimeout, 6400u);
-            p_phase[g] ^= 1u;
+          const bool more = j + 1 < tiles;
+          if (more) {
+            ok = wait(bar_full + 8 * slot, phase, khd::kStatusTmaWaitTimeout, 6500u);
             if (!ok) break;
+          }
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (g >= groups) break;
+            ok = wait(bar_p + 8 * g, p_phase[g], khd::kStatusEpilogueWaitTimeout, 6400u);
+            if (!ok) break;
+            khd::tc_fence_after_sync();
             if (leader) {
 #pragma unroll
               for (int i = 0; i < kKeys / 16; ++i) // 16 keys: 8 columns of P, two groups of 8 rows of V
-                umma_ts(tmem + 256 + g * 128, tmem + g * 128 + i * 8, umma_desc_mn128(v_tile + i * 2048, kHalfBytes), idesc_o, j != 0 || i != 0);
+                umma_ts(tmem + 256 + g * 128, tmem + g * 128 + i * 8, v + i * 128, idesc_o, j != 0 || i != 0);
               if (!more) khd::umma_commit(bar_o + 8 * g);
               if (g == groups - 1) khd::umma_commit(bar_empty + 8 * v_slot);
             }
             __syncwarp();
-            if (more) {
-              if (g == 0) {
-                ok = wait(bar_full + 8 * slot, phase, khd::kStatusTmaWaitTimeout, 6500u);
-                if (!ok) break;
-              }
-              issue_s(g, smem_ring + slot * Cfg::kTileBytes);
-              if (g == groups - 1) {
-                if (leader) khd::umma_commit(bar_empty + 8 * slot);
-                __syncwarp();
-              }
-            }
+            p_phase[g] ^= 1u;
+            if (more) issue_s(g, slot, j + 2 == tiles, g == groups - 1);
           }
           if (more) advance();
+        }
+      }
+    }
+    else if (warp >= kQueryWarp && warp < kQueryWarp + kQueryWarps) {
+      // ---- queries: Q_g of the next item goes in as soon as the last S_g of this one is done. 16-byte chunk c of
+      //      row x lies at chunk c ^ (x % 8) of its 128 bytes (the swizzle a TMA copy would have written). ----
+      uint32_t phase[2] = {1, 1};
+      bool ok = true;
+      while (ok && walker.next(P, k)) {
+        if (k.tiles == 0) continue;
+        for (int g = 0; g < 2 && g * kTileRows < k.rows && ok; ++g) {
+          ok = khd::mbar_wait(bar_q_free + 8 * g, phase[g], &s_abort, P.status, khd::kStatusEmptyWaitTimeout, 6800u);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          phase[g] ^= 1u;
+          constexpr int kChunks = kDim / 8;
+#pragma unroll 4
+          for (int i = 0; i < kTileRows * kChunks / (32 * kQueryWarps); ++i) {
+            const int idx = (i * kQueryWarps + warp - kQueryWarp) * 32 + lane, x = idx / kChunks, c = idx % kChunks;
+            const bool real = g * kTileRows + x < k.rows && c * 8 < P.head_dim;
+            const int qr = k.row0 + (real ? g * kTileRows + x : 0), qt = qr / P.group;
+            const T *src = reinterpret_cast<const T *>(P.q) + (k.s.q0 + qt) * P.q_token + (k.h * P.group + qr - qt * P.group) * P.q_head +
+                           (real ? c * 8 : 0);
+            const uint32_t dst = smem_q + g * Cfg::kTileBytes + (c >> 3) * kHalfBytes + x * 128 + (((c & 7) ^ (x & 7)) << 4);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_async_shared();
+          warp_arrive(bar_q + 8 * g);
         }
       }
     }
@@ -360,25 +424,6 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
       const int see_lo = first > 0 ? static_cast<int>(min(first, static_cast<int64_t>(k.s.kv))) : 0;
       const bool idle = quad * 32 >= rows_here; // no row of this warp is real: its lanes of P may hold anything
       float m = -INFINITY, l = 0.f;             // reference and sum, in exp2 units
-      if (k.tiles > 0) {
-        // Q_g: the warp's 32 rows, 16-byte chunk c of row x at chunk c ^ (x % 8) of its 128 bytes
-        constexpr int kChunks = kDim / 8;
-#pragma unroll 4
-        for (int i = 0; i < kChunks; ++i) {
-          const int idx = i * 32 + lane, x = idx / kChunks, c = idx % kChunks;
-          const int rr = g * kTileRows + quad * 32 + x;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (rr < k.rows && c * 8 < P.head_dim) {
-            const int qr = k.row0 + rr, qt = qr / P.group;
-            v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(P.q) + (k.s.q0 + qt) * P.q_token +
-                                                 (k.h * P.group + qr - qt * P.group) * P.q_head + c * 8);
-          }
-          const uint32_t dst = smem_q + g * Cfg::kTileBytes + (c >> 3) * kHalfBytes + (quad * 32 + x) * 128 + (((c & 7) ^ (x & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-        }
-        fence_async_shared();
-        khd::mbar_arrive(bar_q + 8 * g);
-      }
       for (int j = 0; j < k.tiles; ++j) {
         ok = khd::mbar_wait(bar_s + 8 * g, s_phase, &s_abort, P.status, khd::kStatusMmaWaitTimeout, 6600u);
         if (!ok) break;
@@ -391,7 +436,8 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
           khd::tmem_ld_wait();
           const int key0 = k.key_a + j * kKeys;
           const int lo = see_lo - key0, hi = see_hi - key0; // seen: lo <= i <= hi
-          if (__any_sync(0xffffffffu, lo > 0 || hi < kKeys - 1)) {
+          const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < kKeys - 1);
+          if (masked) {
 #pragma unroll
             for (int i = 0; i < kKeys; ++i)
               if (i < lo || i > hi) s[i] = 0xff800000u; // -inf
@@ -400,12 +446,10 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
 #pragma unroll
           for (int i = 0; i < kKeys; i += 8)
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              top4[x] = fmaxf(top4[x], fmaxf(__uint_as_float(s[i + 2 * x]), __uint_as_float(s[i + 2 * x + 1])));
-          const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * P.scale_log2;
-          const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
-          if (__any_sync(0xffffffffu, raise)) {
-            const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.f : m_new;
+            for (int x = 0; x < 4; ++x) top4[x] = max3_nan(top4[x], __uint_as_float(s[i + 2 * x]), __uint_as_float(s[i + 2 * x + 1]));
+          const float top = max3_nan(max3_nan(top4[0], top4[1], top4[2]), top4[3], -INFINITY) * P.scale_log2;
+          if (__any_sync(0xffffffffu, !(top <= m + kLazy))) { // true of a NaN, which stays in m
+            const float m_new = max3_nan(m, top, -INFINITY), ref = m_new == -INFINITY ? 0.f : m_new;
             const float f = khd::exp2_approx(m - ref);
             m = m_new;
             l *= f;
@@ -423,7 +467,7 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
           }
           const float ref = m == -INFINITY ? 0.f : m;
           const float2 f2 = make_float2(P.scale_log2, P.scale_log2), off2 = make_float2(-ref, -ref);
-          float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int i = 0; i < kKeys / 32; ++i) {
             uint32_t p[16];
@@ -431,16 +475,16 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
             for (int x = 0; x < 16; ++x) {
               const float2 e = __ffma2_rn(make_float2(__uint_as_float(s[32 * i + 2 * x]), __uint_as_float(s[32 * i + 2 * x + 1])), f2, off2);
               const float2 v = make_float2(khd::exp2_approx(e.x), khd::exp2_approx(e.y));
-              sum2[x & 1] = __fadd2_rn(sum2[x & 1], v);
+              sum[x & 1] = __fadd2_rn(sum[x & 1], v);
               p[x] = Types<T>::pack(v.x, v.y);
             }
             tmem_st_32x16(t_s + 16 * i, p);
           }
-          l += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_st_wait();
         }
         khd::tc_fence_before_sync();
-        khd::mbar_arrive(bar_p + 8 * g);
+        warp_arrive(bar_p + 8 * g);
       }
       if (!ok) break;
       // ---- the finished rows of this tile ------------------------------------------------------------------
@@ -509,9 +553,9 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
                                          const __grid_constant__ khd::TensorMap tm_v, int box_rows) {                      \
     chunk_body<T, dim>(P, tm_k, tm_v, box_rows);                                                                          \
   }                                                                                                                       \
-  extern "C" __global__ void __launch_bounds__(128) paged_attention_chunk_combine_##suffix##_##dim(                       \
+  extern "C" __global__ void __launch_bounds__(256) paged_attention_chunk_combine_##suffix##_##dim(                       \
       const __grid_constant__ PagedParams P) {                                                                            \
-    khp::combine_rows<128, kRows, kKeys, dim>(P, [&](int token, int head, int c, float v) {                               \
+    khp::combine_rows<kRows, dim>(P, [&](int token, int head, int c, float v) {                               \
       reinterpret_cast<T *>(P.o)[token * P.o_token + head * P.o_head + c] = Types<T>::from(v);                            \
     });                                                                                                                   \
   }

@@ -32,7 +32,7 @@ struct PagedParams {
   int64_t table_stride;
   const int32_t *q_start, *kv_len;
   float *lse, *partial_o;
-  void *partial_ml;
+  void *partial_ml, *split_items;
   uint32_t *status;
   int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, table_width, num_pages;
   int32_t causal, window;
@@ -77,7 +77,7 @@ int64_t worker_count(const kh_paged_attention_args &a, int rows, int unit, int p
   const int64_t most = per_sm * std::min(sms, kMaxSms);
   return std::min<int64_t>(most, std::max<int64_t>(1, (items * units + kMinUnits - 1) / kMinUnits));
 }
-int64_t workspace_for(int64_t workers, int rows, int dim) { return 2 * workers * rows * (dim * 4 + 8); }
+int64_t workspace_for(int64_t workers, int rows, int dim) { return workers * (2 * rows * (dim * 4 + 8) + 32); }
 
 std::string check_stride(const char *name, const void *data, std::initializer_list<std::pair<int64_t, int64_t>> strides, int32_t head_dim,
                          int size, bool output) {
@@ -192,7 +192,9 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
   const auto workers = [&](int rows, int unit, int per_sm) {
     const int64_t n = worker_count(a, rows, unit, per_sm, sms);
     p.workers = static_cast<int32_t>(n);
-    p.partial_ml = static_cast<char *>(a.workspace) + 2 * n * rows * s.dim * 4;
+    char *base = static_cast<char *>(a.workspace); // rows, notes of split items, (max, sum) pairs
+    p.split_items = base + 2 * n * rows * s.dim * 4;
+    p.partial_ml = base + 2 * n * rows * s.dim * 4 + n * 32;
     return static_cast<unsigned>(n);
   };
   const int64_t all_rows = a.tokens * p.group;
@@ -231,9 +233,9 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
     const size_t smem = static_cast<size_t>(2 + stages) * kChunkKeys * s.dim * 2 + 1024;
     if (auto r = launch("paged_attention_chunk", "paged_attention_chunk_" + suffix, {n, 1, 1}, 512, smem, {maps[0], maps[1]}, box_rows); !r) return r;
     if (n > 1) {
-      // an item is split where a worker's stretch begins inside it: 32 rows of it per block
-      const unsigned y = static_cast<unsigned>((std::min<int64_t>(kChunkRows, all_rows) + 31) / 32);
-      if (auto r = launch("paged_attention_chunk", "paged_attention_chunk_combine_" + suffix, {n - 1, y, 1}, 128, 0, {}, 0); !r) return r;
+      // an item is split where a worker's stretch begins inside it: 16 rows of it per block
+      const unsigned y = static_cast<unsigned>((std::min<int64_t>(kChunkRows, all_rows) + 15) / 16);
+      if (auto r = launch("paged_attention_chunk", "paged_attention_chunk_combine_" + suffix, {n - 1, y, 1}, 256, 0, {}, 0); !r) return r;
     }
     if (alone) return {};
     p.rows_above = 0, p.rows_upto = kRows;
