@@ -39,7 +39,7 @@ struct PagedParams {
   float2 *partial_ml;
   struct SplitItem *split_items; // [workers]
   uint32_t *status;
-  int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, table_width, num_pages;
+  int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, page_shift, table_width, num_pages; // page_size = 2^page_shift, or page_shift < 0
   int32_t causal, window;  // window 0: none
   int32_t workers, min_units;
   int32_t rows_above, rows_upto; // sequences with rows in (rows_above, rows_upto] are this launch's

@@ -26,6 +26,7 @@ using khp::PagedParams;
 constexpr int kRows = 16;    // rows of an item
 constexpr int kKeys = 16;    // keys of a warp's step
 constexpr int kStages = 3;   // ring of a warp
+constexpr float kLazy = 8.f;
 
 template <typename T, int kDim> struct Config {
   static constexpr int kRowBytes = kDim * static_cast<int>(sizeof(T));
@@ -37,12 +38,15 @@ template <typename T, int kDim> struct Config {
   static constexpr int kPitch = kRowBytes + 16; // bytes between rows: ldmatrix and fp32 reads without bank conflicts
   static constexpr int kTile = kKeys * kPitch;
   static constexpr int kRing = kStages * 2 * kTile;
-  static constexpr int kSmem = kWarps * kRing;
+  static constexpr int kSmem = kWarps * kRing + (sizeof(T) == 4 ? kTile : 0); // fp32 queries lie behind the rings
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-// 16 bytes global -> shared; nothing is read and zeros are written when !valid
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool valid) {
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// nothing is read and zeros are written when !valid
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void *src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -113,23 +117,42 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// The 16-row query tile as A fragments. 16-bit: k-step s holds rows (g, g + 8) x columns 16 s + 2c (+1) and
-// + 8; fp32: k-step s holds columns 8 s + c and + 4 (g = lane / 4, c = lane % 4). Zeros outside rows and head_dim.
+// The 16-row query tile as A fragments. 16-bit types keep them in registers: k-step s holds rows (g, g + 8) x columns
+// 16 s + 2c (+1) and + 8 (g = lane / 4, c = lane % 4). fp32 rows are twice that: they lie in shared memory, padded like
+// the keys, and a k-step's fragment (columns 8 s + c and + 4) is one ldmatrix. Zeros outside rows and head_dim.
 template <typename T, int kDim> struct Queries {
-  static constexpr bool k16 = sizeof(T) == 2;
-  static constexpr int kStepsK = k16 ? kDim / 16 : kDim / 8;
+  static constexpr int kStepsK = kDim / 16;
   uint32_t a[kStepsK][4];
-  __device__ __forceinline__ void load(const PagedParams &P, const T *row0, const T *row1) {
+  __device__ __forceinline__ void load(const PagedParams &P, const T *row0, const T *row1, uint32_t) {
     const int c = threadIdx.x & 3;
 #pragma unroll
     for (int s = 0; s < kStepsK; ++s) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const T *row = j & 1 ? row1 : row0;
-        const int col = k16 ? 16 * s + 2 * c + (j >> 1) * 8 : 8 * s + c + (j >> 1) * 4;
+        const int col = 16 * s + 2 * c + (j >> 1) * 8;
         a[s][j] = row != nullptr && col < P.head_dim ? *reinterpret_cast<const uint32_t *>(row + col) : 0u;
       }
     }
+  }
+};
+template <int kDim> struct Queries<float, kDim> {
+  static constexpr int kStepsK = kDim / 8;
+  uint32_t at;
+  // Every warp calls this; the block has passed a barrier since the last use, and passes one before the next.
+  __device__ __forceinline__ void load(const PagedParams &P, const float *row0, const float *row1, uint32_t tile) {
+    constexpr int kPitch = Config<float, kDim>::kPitch, kWarps = Config<float, kDim>::kWarps;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int c = (warp * 4 + (lane & 3)) * 4; c < kDim; c += kWarps * 16) // this warp's share of the lane's two rows
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float *row = x ? row1 : row0;
+        const float4 v = row != nullptr && c < P.head_dim ? *reinterpret_cast<const float4 *>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(tile + ((lane >> 2) + 8 * x) * kPitch + c * 4), "f"(v.x), "f"(v.y),
+                     "f"(v.z), "f"(v.w)
+                     : "memory");
+      }
+    at = tile + (lane & 15) * kPitch + (lane >> 4) * 16;
   }
 };
 
@@ -152,8 +175,9 @@ __device__ __forceinline__ void score_tile(const Queries<T, kDim> &q, uint32_t t
       mma16<T>(s[0], q.a[k], b[0], b[1]);
       mma16<T>(s[1], q.a[k], b[2], b[3]);
     } else {
-      uint32_t hi[4], lo[4];
-      split_tf32(q.a[k], hi, lo);
+      uint32_t a[4], hi[4], lo[4];
+      ldsm4(a, q.at + k * 32);
+      split_tf32(a, hi, lo);
       mma8_fp32(s[0], hi, lo, b[0], b[1]);
       mma8_fp32(s[1], hi, lo, b[2], b[3]);
     }
@@ -204,7 +228,7 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t ring = smem_addr(smem) + warp * Cfg::kRing;
   if (P.head_dim < kDim) { // columns that no copy writes count as zeros
-    for (int i = threadIdx.x * 16; i < Cfg::kSmem; i += kThreads * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x * 16; i < kWarps * Cfg::kRing; i += kThreads * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
   khd::grid_dependency_wait();
@@ -224,6 +248,7 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
   if (threadIdx.x == 0) khp::note_split<Cut>(P, line, w, at, b, start);
   khp::Sequence s = khp::sequence<Cut>(P, b);
 
+  const bool whole_steps = P.page_size % kKeys == 0; // a step's keys lie in one page
   const int chunks_per_row = P.head_dim * static_cast<int>(sizeof(T)) / 16; // 16-byte pieces that exist
   while (at < until) {
     int64_t size = static_cast<int64_t>(s.blocks) * s.span * P.k_heads;
@@ -265,8 +290,13 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
       const int64_t first = P.window > 0 ? static_cast<int64_t>(past) + t - P.window + 1 : 0;
       see_lo[i] = static_cast<int>(first > 0 ? first : 0);
     }
+    // what all real rows of the warp's tile see: a step inside needs no mask (rows that are not real are not stored)
+    const int all_hi = P.causal ? past + t_first : s.kv - 1;
+    const int64_t last_lo = P.window > 0 ? static_cast<int64_t>(past) + t_last - P.window + 1 : 0;
+    const int all_lo = static_cast<int>(min(max(last_lo, static_cast<int64_t>(0)), static_cast<int64_t>(s.kv)));
     Queries<T, kDim> q;
-    q.load(P, q_row[0], q_row[1]);
+    q.load(P, q_row[0], q_row[1], smem_addr(smem) + kWarps * Cfg::kRing);
+    if (sizeof(T) == 4) __syncthreads();
 
     float o[kDim / 8][4];
 #pragma unroll
@@ -279,33 +309,59 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
     const char *k_base = P.k + static_cast<int64_t>(h) * P.k_head * sizeof(T), *v_base = P.v + static_cast<int64_t>(h) * P.v_head * sizeof(T);
     const int steps = key_b > key_a ? ((key_b - key_a + kUnit - 1) / kUnit) * Cfg::kSteps : 0;
     const auto key_of = [&](int i) { return key_a + (i / Cfg::kSteps) * kUnit + (i % Cfg::kSteps * kWarps + warp) * kKeys; };
-    // lane r < 16 looks up the page of row r one step ahead of its use
+    constexpr int kChunks = Cfg::kRowBytes / 16;
+    // The page of the step after the one being fetched is looked up ahead of its use: one for the step where pages
+    // are whole steps, else lane r < 16 looks up row r's.
     int page_next = 0;
     const auto look_up = [&](int i) {
-      const int key = key_of(i) + (lane & 15);
-      page_next = i < steps && key < key_b ? __ldg(table + key / P.page_size) : 0;
+      const int key = key_of(i) + (whole_steps ? 0 : lane & 15);
+      page_next = i < steps && key < key_b ? __ldg(table + (P.page_shift >= 0 ? key >> P.page_shift : key / P.page_size)) : 0;
     };
     const auto issue = [&](int i) {
-      if (i < steps && key_of(i) < key_b) {
-        const int key0 = key_of(i), key = key0 + (lane & 15);
-        bool good = key < key_b && key >= lo_key; // evicted keys before every row's window are not read
-        int page = page_next;
-        if (good && (page < 0 || page >= P.num_pages)) {
-          khd::report_status(P.status, khd::kStatusBadPage, static_cast<uint32_t>(b));
-          good = false;
-        }
-        const int slot = key % P.page_size;
-        const int64_t k_off = good ? (page * P.k_page + slot * P.k_slot) * static_cast<int64_t>(sizeof(T)) : -1;
-        const int64_t v_off = good ? (page * P.v_page + slot * P.v_slot) * static_cast<int64_t>(sizeof(T)) : -1;
-        const uint32_t k_tile = ring + (i % kStages) * 2 * Cfg::kTile, v_tile = k_tile + Cfg::kTile;
-        constexpr int kChunks = Cfg::kRowBytes / 16;
+      const int key0 = key_of(i);
+      if (i < steps && key0 < key_b) {
+        const uint32_t k_tile = ring + (i % kStages) * 2 * Cfg::kTile;
+        if (whole_steps && key0 >= lo_key && key0 + kKeys <= key_b && static_cast<unsigned>(page_next) < static_cast<unsigned>(P.num_pages)) {
+          // sixteen rows of one page, all of them wanted: copy j takes the rows kStride further on
+          constexpr int kStride = kChunks < 32 ? 32 / kChunks : 1;
+          const int slot = (P.page_shift >= 0 ? key0 & (P.page_size - 1) : key0 % P.page_size) + lane / kChunks;
+          const char *kp = k_base + (page_next * P.k_page + slot * P.k_slot) * static_cast<int64_t>(sizeof(T)) + lane % kChunks * 16;
+          const char *vp = v_base + (page_next * P.v_page + slot * P.v_slot) * static_cast<int64_t>(sizeof(T)) + lane % kChunks * 16;
+          const uint32_t dst = k_tile + lane / kChunks * Cfg::kPitch + lane % kChunks * 16;
+          const int64_t k_step = kStride * P.k_slot * static_cast<int64_t>(sizeof(T)), v_step = kStride * P.v_slot * static_cast<int64_t>(sizeof(T));
+          if (lane % kChunks < chunks_per_row) {
 #pragma unroll
-        for (int j = 0; j < kKeys * kChunks / 32; ++j) {
-          const int idx = j * 32 + lane, row = idx / kChunks, c = idx % kChunks;
-          const int64_t ko = __shfl_sync(0xffffffffu, k_off, row), vo = __shfl_sync(0xffffffffu, v_off, row);
-          if (c < chunks_per_row) {
-            copy16(k_tile + row * Cfg::kPitch + c * 16, ko >= 0 ? k_base + ko + c * 16 : k_base, ko >= 0);
-            copy16(v_tile + row * Cfg::kPitch + c * 16, vo >= 0 ? v_base + vo + c * 16 : v_base, vo >= 0);
+            for (int j = 0; j < kKeys / kStride; ++j) {
+#pragma unroll
+              for (int x = 0; x < (kChunks + 31) / 32; ++x) { // rows of more than 32 pieces take two copies
+                if (x > 0 && lane + 32 * x >= chunks_per_row) break;
+                copy16(dst + j * kStride * Cfg::kPitch + x * 512, kp + x * 512);
+                copy16(dst + Cfg::kTile + j * kStride * Cfg::kPitch + x * 512, vp + x * 512);
+              }
+              kp += k_step;
+              vp += v_step;
+            }
+          }
+        } else {
+          const int key = key0 + (lane & 15);
+          bool good = key < key_b && key >= lo_key; // evicted keys before every row's window are not read
+          const int page = page_next;
+          if (good && (page < 0 || page >= P.num_pages)) {
+            khd::report_status(P.status, khd::kStatusBadPage, static_cast<uint32_t>(b));
+            good = false;
+          }
+          const int slot = key % P.page_size;
+          const int64_t k_off = good ? (page * P.k_page + slot * P.k_slot) * static_cast<int64_t>(sizeof(T)) : -1;
+          const int64_t v_off = good ? (page * P.v_page + slot * P.v_slot) * static_cast<int64_t>(sizeof(T)) : -1;
+          const uint32_t v_tile = k_tile + Cfg::kTile;
+#pragma unroll 4
+          for (int j = 0; j < kKeys * kChunks / 32; ++j) {
+            const int idx = j * 32 + lane, row = idx / kChunks, c = idx % kChunks;
+            const int64_t ko = __shfl_sync(0xffffffffu, k_off, row), vo = __shfl_sync(0xffffffffu, v_off, row);
+            if (c < chunks_per_row) {
+              copy16_or_zero(k_tile + row * Cfg::kPitch + c * 16, ko >= 0 ? k_base + ko + c * 16 : k_base, ko >= 0);
+              copy16_or_zero(v_tile + row * Cfg::kPitch + c * 16, vo >= 0 ? v_base + vo + c * 16 : v_base, vo >= 0);
+            }
           }
         }
       }
@@ -325,26 +381,39 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
       const uint32_t k_tile = ring + (i % kStages) * 2 * Cfg::kTile;
       float sc[2][4];
       score_tile<T, kDim>(q, k_tile, sc);
-      float top[2] = {m[0], m[1]};
+      float top[2] = {-INFINITY, -INFINITY};
+      if (key0 + kKeys - 1 <= all_hi && key0 >= all_lo) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = key0 + 8 * t + 2 * (lane & 3) + (j & 1), i2 = j >> 1;
-          const bool seen = key <= see_hi[i2] && key >= see_lo[i2];
-          sc[t][j] = seen ? sc[t][j] * P.scale_log2 : -INFINITY;
-          top[i2] = fmaxf(top[i2], sc[t][j]);
-        }
+          for (int j = 0; j < 4; ++j) {
+            sc[t][j] *= P.scale_log2;
+            top[j >> 1] = fmaxf(top[j >> 1], sc[t][j]);
+          }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = key0 + 8 * t + 2 * (lane & 3) + (j & 1), i2 = j >> 1;
+            const bool seen = key <= see_hi[i2] && key >= see_lo[i2];
+            sc[t][j] = seen ? sc[t][j] * P.scale_log2 : -INFINITY;
+            top[i2] = fmaxf(top[i2], sc[t][j]);
+          }
+      }
 #pragma unroll
       for (int i2 = 0; i2 < 2; ++i2) {
         top[i2] = fmaxf(top[i2], __shfl_xor_sync(0xffffffffu, top[i2], 1));
         top[i2] = fmaxf(top[i2], __shfl_xor_sync(0xffffffffu, top[i2], 2));
       }
-      if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+      // The reference is raised when a maximum has outgrown it by 2^8 (the rows' first keys among that): until then
+      // the exponentials reach at most 2^8, and the output need not be touched.
+      if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
 #pragma unroll
         for (int i2 = 0; i2 < 2; ++i2) {
-          const float f = exp2f(m[i2] - (top[i2] == -INFINITY ? 0.f : top[i2]));
-          m[i2] = top[i2];
+          const float m_new = fmaxf(m[i2], top[i2]);
+          const float f = khd::exp2_approx(m[i2] - (m_new == -INFINITY ? 0.f : m_new));
+          m[i2] = m_new;
           l[i2] *= f;
 #pragma unroll
           for (int n = 0; n < kDim / 8; ++n) {
@@ -353,13 +422,13 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
           }
         }
       }
-      // a row that has seen no key yet keeps max -inf; its exponentials are taken against 0 and are all 0
+      // a row that has seen no key yet keeps reference -inf; its exponentials are taken against 0 and are all 0
       const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          sc[t][j] = exp2f(sc[t][j] - ref[j >> 1]);
+          sc[t][j] = khd::exp2_approx(sc[t][j] - ref[j >> 1]);
           l[j >> 1] += sc[t][j];
         }
       value_tile<T, kDim>(sc, k_tile + Cfg::kTile, o);
@@ -424,7 +493,7 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
     }
     __syncthreads(); // the scratch becomes rings again
     if (P.head_dim < kDim) { // and their unwritten columns zeros
-      for (int i = threadIdx.x * 16; i < Cfg::kSmem; i += kThreads * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
+      for (int i = threadIdx.x * 16; i < kWarps * Cfg::kRing; i += kThreads * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
       __syncthreads();
     }
     at = until < end ? until : end;

@@ -3,6 +3,7 @@
 // name takes fp32 buffers of one layout.
 #include "executor.hpp"
 
+#include <bit>
 #include <climits>
 #include <cmath>
 #include <string>
@@ -34,7 +35,7 @@ struct PagedParams {
   float *lse, *partial_o;
   void *partial_ml, *split_items;
   uint32_t *status;
-  int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, table_width, num_pages;
+  int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, page_shift, table_width, num_pages;
   int32_t causal, window;
   int32_t workers, min_units;
   int32_t rows_above, rows_upto;
@@ -53,7 +54,7 @@ Shape kernel_shape(int32_t dtype, int32_t head_dim) {
   const int row_bytes = s.dim * element_size(dtype);
   s.warps = row_bytes <= 512 ? 4 : 2;
   s.per_sm = row_bytes <= 128 ? 3 : row_bytes <= 256 ? 2 : 1;
-  s.smem = static_cast<size_t>(s.warps) * 3 * 2 * 16 * (row_bytes + 16);
+  s.smem = static_cast<size_t>(s.warps * 3 * 2 + (dtype == KH_F32 ? 1 : 0)) * 16 * (row_bytes + 16);
   return s;
 }
 
@@ -167,7 +168,8 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
   p.status = ex.status_word();
   p.tokens = static_cast<int32_t>(a.tokens), p.batch = a.batch, p.q_heads = a.q_heads, p.k_heads = a.k_heads;
   p.group = a.q_heads / a.k_heads, p.head_dim = a.head_dim;
-  p.page_size = a.page_size, p.table_width = a.table_width, p.num_pages = static_cast<int32_t>(a.num_pages);
+  p.page_size = a.page_size, p.page_shift = (a.page_size & (a.page_size - 1)) == 0 ? std::countr_zero(static_cast<unsigned>(a.page_size)) : -1;
+  p.table_width = a.table_width, p.num_pages = static_cast<int32_t>(a.num_pages);
   p.causal = a.causal, p.window = a.window;
   p.min_units = kMinUnits;
   p.scale_log2 = a.scale * 1.4426950408889634f;
