@@ -402,7 +402,7 @@ class Context:
     # These take torch tensors and read shapes, strides and types from them.
     def _on_device(self, t, name: str, dtype: str | None = None, size: int | None = None) -> int:
         """Address of a contiguous vector on this context's device, of `dtype` and `size` values."""
-        if not t.is_cuda or t.get_device() != self._ordinal:
+        if t.get_device() != self._ordinal:  # -1 for a tensor in host memory
             _refuse(f"'{name}' must be on device {self._ordinal} of this context, got {t.device}")
         if dtype is not None and str(t.dtype) != dtype:
             _refuse(f"'{name}' must be {dtype}, got {t.dtype}")
@@ -414,7 +414,7 @@ class Context:
 
     def _rows(self, t, name: str, shape, code: int) -> HeadRows:
         """A [tokens, heads, head_dim] tensor as rows: any strides but the last, which must be 1."""
-        if not t.is_cuda or t.get_device() != self._ordinal:
+        if t.get_device() != self._ordinal:  # -1 for a tensor in host memory
             _refuse(f"'{name}' must be on device {self._ordinal} of this context, got {t.device}")
         if t.shape != shape:
             _refuse(f"'{name}' must have shape {tuple(shape)}, got {tuple(t.shape)}")
@@ -427,7 +427,7 @@ class Context:
 
     def _cache(self, t, name: str, shape, code: int) -> PagedRows:
         """A [pages, page_size, heads, head_dim] tensor as a paged cache: any strides but the last."""
-        if not t.is_cuda or t.get_device() != self._ordinal:
+        if t.get_device() != self._ordinal:  # -1 for a tensor in host memory
             _refuse(f"'{name}' must be on device {self._ordinal} of this context, got {t.device}")
         if t.dim() != 4 or tuple(t.shape) != shape:
             _refuse(f"'{name}' must have shape {shape}, got {tuple(t.shape)}")
@@ -521,7 +521,7 @@ class Context:
         pages, page_size, k_heads, _ = k_cache.shape
         if page_table.dim() != 2 or str(page_table.dtype) != "torch.int32" or page_table.stride(1) != 1:
             _refuse("'page_table' must be int32 [batch, width] with contiguous rows")
-        if not page_table.is_cuda or page_table.get_device() != self._ordinal:
+        if page_table.get_device() != self._ordinal:
             _refuse(f"'page_table' must be on device {self._ordinal} of this context, got {page_table.device}")
         batch, width = page_table.shape
         shape = (pages, page_size, k_heads, head_dim)

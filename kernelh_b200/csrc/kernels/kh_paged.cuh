@@ -42,6 +42,7 @@ struct PagedParams {
   int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, page_shift, table_width, num_pages; // page_size = 2^page_shift, or page_shift < 0
   int32_t causal, window;  // window 0: none
   int32_t workers, min_units;
+  int32_t whole; // 1: a worker takes the items that begin in its stretch, whole; nothing is split
   int32_t rows_above, rows_upto; // sequences with rows in (rows_above, rows_upto] are this launch's
   float scale_log2;              // scale * log2(e): scores are kept in exp2 units
 };
@@ -89,14 +90,22 @@ template <typename G> __device__ __forceinline__ int64_t sequence_span(const Pag
 // neighbours in that order adds up to the same.
 __device__ __forceinline__ int block_of(int i, int blocks) { return i & 1 ? blocks - 1 - (i >> 1) : i >> 1; }
 
-// The whole line and the place of one unit on it, worked out by the block together.
+// 64-bit quotients cost a hundred instructions; nearly all of these fit 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int32_t b) {
+  return a < (int64_t{1} << 31) ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
+// The whole line, dealt out evenly: worker w's stretch begins at stretch(w) (w = workers: the line's end).
 struct Line {
-  int64_t total;
-  int workers; // of which the first `workers` have any work
+  int64_t total, share;
+  int workers, rest; // of which the first `workers` have any work
+  __device__ __forceinline__ int64_t stretch(int w) const {
+    return share * w + static_cast<int64_t>(static_cast<uint32_t>(rest) * static_cast<uint32_t>(w) / static_cast<uint32_t>(workers)); // both below 2^15
+  }
 };
 template <int kThreads> struct LineScratch {
   int64_t warp_sum[kThreads / 32];
-  int64_t total, start;
+  int64_t start;
   int b;
 };
 
@@ -121,42 +130,38 @@ template <int kThreads> __device__ __forceinline__ int64_t block_scan(int64_t v,
   return all;
 }
 
-template <int kThreads, typename G>
-__device__ __forceinline__ Line measure_line(const PagedParams &P, LineScratch<kThreads> &s) {
+// The block works out the line together, and where worker w's stretch begins: in sequence scratch.b, which begins
+// at scratch.start (both stay there). The order is that of the sequences; a thread takes one, of each kThreads.
+template <int kThreads, typename G> __device__ __forceinline__ Line lay_line(const PagedParams &P, int w, LineScratch<kThreads> &scratch) {
+  Line line;
   int64_t mine = 0, inclusive;
   for (int b = threadIdx.x; b < P.batch; b += kThreads) mine += sequence_span<G>(P, b);
-  Line line;
-  line.total = block_scan<kThreads>(mine, inclusive, s.warp_sum);
-  const int64_t most = (line.total + P.min_units - 1) / P.min_units;
+  line.total = block_scan<kThreads>(mine, inclusive, scratch.warp_sum);
+  const int64_t most = quotient(line.total + P.min_units - 1, P.min_units);
   line.workers = static_cast<int>(most < P.workers ? most : P.workers);
-  return line;
-}
-// Where worker w's stretch begins (w = workers: the end of the line).
-__device__ __forceinline__ int64_t stretch(const Line &line, int w) {
-  return line.total / line.workers * w + line.total % line.workers * w / line.workers;
-}
-// The sequence that unit `at` (< total) belongs to, and where that sequence starts on the line.
-template <int kThreads, typename G>
-__device__ __forceinline__ void locate(const PagedParams &P, int64_t at, LineScratch<kThreads> &s, int &b_out, int64_t &start) {
+  if (w >= line.workers) return line;
+  line.share = quotient(line.total, line.workers);
+  line.rest = static_cast<int>(line.total - line.share * line.workers);
+  const int64_t at = line.stretch(w);
   int64_t before = 0;
-  for (int base = 0; base < P.batch; base += kThreads) {
+  for (int base = 0;; base += kThreads) { // with more sequences than threads, again group by group
     const int b = base + static_cast<int>(threadIdx.x);
-    const int64_t mine = b < P.batch ? sequence_span<G>(P, b) : 0;
-    int64_t inclusive;
-    const int64_t all = block_scan<kThreads>(mine, inclusive, s.warp_sum);
+    int64_t all = line.total;
+    if (P.batch > kThreads) {
+      mine = b < P.batch ? sequence_span<G>(P, b) : 0;
+      all = block_scan<kThreads>(mine, inclusive, scratch.warp_sum);
+    }
     if (at < before + all) {
-      if (mine > 0 && at >= before + inclusive - mine && at < before + inclusive) {
-        s.b = b;
-        s.start = before + inclusive - mine;
+      if (at >= before + inclusive - mine && at < before + inclusive) {
+        scratch.b = b;
+        scratch.start = before + inclusive - mine;
       }
       break;
     }
     before += all;
   }
   __syncthreads();
-  b_out = s.b;
-  start = s.start;
-  __syncthreads();
+  return line;
 }
 
 // The item that worker w's stretch begins inside of, if no earlier stretch does (parts 0 otherwise). Its part 0
@@ -165,21 +170,21 @@ struct alignas(32) SplitItem {
   int32_t q0, row0, rows, h, parts; // rows: of the item
 };
 __device__ __forceinline__ int64_t part_slot(int w, int p) { return 2 * static_cast<int64_t>(w - 1 + p) + (p == 0 ? 1 : 0); }
-// One thread of worker w notes it down. `at`: where the stretch begins, in sequence b, which begins at `start`.
-template <typename G>
-__device__ __forceinline__ void note_split(const PagedParams &P, const Line &line, int w, int64_t at, int b, int64_t start) {
+// One thread of worker w notes it down. The stretch begins in sequence b, which begins at `start`.
+template <typename G> __device__ __forceinline__ void note_split(const PagedParams &P, const Line &line, int w, int b, int64_t start) {
   SplitItem x{};
   if (w > 0 && w < line.workers) {
     const Sequence s = sequence<G>(P, b);
-    const int64_t item = (at - start) / s.span; // head * blocks + place of the row block
+    const int64_t at = line.stretch(w);
+    const int64_t item = quotient(at - start, s.span); // head * blocks + place of the row block
     const int64_t begin = start + item * s.span, end = begin + s.units;
-    if (begin < at && at < end && begin >= stretch(line, w - 1)) {
+    if (begin < at && at < end && begin >= line.stretch(w - 1)) {
       x.q0 = s.q0;
-      x.h = static_cast<int>(item / s.blocks);
+      x.h = static_cast<int>(quotient(item, s.blocks));
       x.row0 = block_of(static_cast<int>(item - static_cast<int64_t>(x.h) * s.blocks), s.blocks) * G::kRows;
       x.rows = min(G::kRows, s.rows - x.row0);
       int last = w; // the last worker with a part
-      while (last + 1 < line.workers && stretch(line, last + 1) < end) ++last;
+      while (last + 1 < line.workers && line.stretch(last + 1) < end) ++last;
       x.parts = last - w + 2;
     }
   }
@@ -201,19 +206,31 @@ template <int kThreads, int kRows, int kDim, typename Store> __device__ __forcei
   float m = -INFINITY, l = 0.f, acc[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int p = warp; p < x.parts; p += kWarps) {
+  constexpr int kAhead = 4; // parts on their way at once
+  float2 mls[kAhead];
+  float ys[kAhead][kPer];
+  const auto fetch = [&](int p, float2 &ml, float (&y)[kPer]) {
+    if (p >= x.parts) return;
     const int64_t at = part_slot(w, p) * kRows + in_block;
-    const float2 ml = P.partial_ml[at];
-    float y[kPer];
+    ml = P.partial_ml[at];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) y[i] = P.partial_o[at * kDim + i * 32 + lane];
+  };
+  for (int p0 = warp; p0 < x.parts; p0 += kAhead * kWarps) {
+#pragma unroll
+   for (int a = 0; a < kAhead; ++a) fetch(p0 + a * kWarps, mls[a], ys[a]);
+#pragma unroll
+   for (int a = 0; a < kAhead; ++a) {
+    if (p0 + a * kWarps >= x.parts) break;
+    const float2 ml = mls[a];
+    const float (&y)[kPer] = ys[a];
     const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
     const float f_old = exp2f(m - ref), f_new = exp2f(ml.x - ref);
     l = l * f_old + ml.y * f_new;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * f_old + y[i] * f_new;
     m = m_new;
+   }
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) s_row[warp][i * 32 + lane] = acc[i];

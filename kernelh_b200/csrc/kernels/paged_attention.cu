@@ -233,20 +233,17 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
   }
   khd::grid_dependency_wait();
   khd::grid_dependents_may_launch();
-  const khp::Line line = khp::measure_line<kThreads, Cut>(P, scratch);
   const int w = blockIdx.x;
+  const khp::Line line = khp::lay_line<kThreads, Cut>(P, w, scratch);
   if (w >= line.workers) {
-    if (threadIdx.x == 0) P.split_items[w] = khp::SplitItem{};
+    if (threadIdx.x == 0 && !P.whole) P.split_items[w] = khp::SplitItem{};
     return;
   }
-  int64_t at = khp::stretch(line, w);
-  const int64_t until = khp::stretch(line, w + 1);
-  const int64_t from = at;
-  int b;
-  int64_t start;
-  khp::locate<kThreads, Cut>(P, at, scratch, b, start);
-  if (threadIdx.x == 0) khp::note_split<Cut>(P, line, w, at, b, start);
+  const int64_t from = line.stretch(w), until = line.stretch(w + 1);
+  int64_t at = from, start = scratch.start;
+  int b = scratch.b;
   khp::Sequence s = khp::sequence<Cut>(P, b);
+  if (P.whole) at = start + khp::quotient(at - start + s.span - 1, s.span) * s.span; // the first item that begins here
 
   const bool whole_steps = P.page_size % kKeys == 0; // a step's keys lie in one page
   const int chunks_per_row = P.head_dim * static_cast<int>(sizeof(T)) / 16; // 16-byte pieces that exist
@@ -257,15 +254,15 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
       s = khp::sequence<Cut>(P, ++b);
       size = static_cast<int64_t>(s.blocks) * s.span * P.k_heads;
     }
-    const int64_t item = (at - start) / s.span;
+    const int64_t item = khp::quotient(at - start, s.span);
     const int64_t begin = start + item * s.span, end = begin + s.span;
     if (at - begin >= s.units) { // what is left of the item is only what stands for its end
       at = end;
       continue;
     }
-    const int h = static_cast<int>(item / s.blocks);
+    const int h = static_cast<int>(khp::quotient(item, s.blocks));
     const int block = khp::block_of(static_cast<int>(item - static_cast<int64_t>(h) * s.blocks), s.blocks);
-    const int unit0 = static_cast<int>(at - begin), unit1 = static_cast<int>(min((until < end ? until : end) - begin, static_cast<int64_t>(s.units)));
+    const int unit0 = static_cast<int>(at - begin), unit1 = P.whole ? s.units : static_cast<int>(min((until < end ? until : end) - begin, static_cast<int64_t>(s.units)));
     const int row0 = block * kRows, rows_here = min(kRows, s.rows - row0);
     // keys that rows of this block see, and the part of them in this stretch
     const int t_first = row0 / P.group, t_last = (row0 + rows_here - 1) / P.group;
@@ -496,12 +493,13 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
       for (int i = threadIdx.x * 16; i < kWarps * Cfg::kRing; i += kThreads * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
       __syncthreads();
     }
-    at = until < end ? until : end;
+    at = until < end && !P.whole ? until : end;
   }
+  if (threadIdx.x == 0 && !P.whole) khp::note_split<Cut>(P, line, w, scratch.b, scratch.start);
 }
 
 template <typename T, int kDim> __device__ __forceinline__ void combine(const PagedParams &P) {
-  khp::combine_row<128, kRows, kDim>(P, [&](int token, int head, int c, float v) {
+  khp::combine_row<256, kRows, kDim>(P, [&](int token, int head, int c, float v) {
     reinterpret_cast<T *>(P.o)[token * P.o_token + head * P.o_head + c] = from_float<T>(v);
   });
 }
@@ -511,7 +509,7 @@ template <typename T, int kDim> __device__ __forceinline__ void combine(const Pa
 #define KH_PAGED(suffix, T, dim)                                                                                              \
   extern "C" __global__ void __launch_bounds__(Config<T, dim>::kThreads)                                                      \
   paged_attention_##suffix##_##dim(const __grid_constant__ PagedParams P) { attention_body<T, dim>(P); }                      \
-  extern "C" __global__ void __launch_bounds__(128) paged_attention_combine_##suffix##_##dim(                                 \
+  extern "C" __global__ void __launch_bounds__(256) paged_attention_combine_##suffix##_##dim(                                 \
       const __grid_constant__ PagedParams P) { combine<T, dim>(P); }
 
 KH_PAGED(f32, float, 64)

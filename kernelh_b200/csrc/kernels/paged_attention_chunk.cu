@@ -154,13 +154,13 @@ struct Walker {
         k.s = khp::sequence<Cut>(P, ++b);
         size = static_cast<int64_t>(k.s.blocks) * k.s.span * P.k_heads;
       }
-      item = (at - start) / k.s.span;
+      item = khp::quotient(at - start, k.s.span);
       begin = start + item * k.s.span, end = begin + k.s.span;
       if (at - begin < k.s.units) break;
       at = end; // what is left of the item is only what stands for its end
     }
     k.b = b;
-    k.h = static_cast<int>(item / k.s.blocks);
+    k.h = static_cast<int>(khp::quotient(item, k.s.blocks));
     const int block = khp::block_of(static_cast<int>(item - static_cast<int64_t>(k.h) * k.s.blocks), k.s.blocks);
     const int unit0 = static_cast<int>(at - begin), unit1 = static_cast<int>(min((until < end ? until : end) - begin, static_cast<int64_t>(k.s.units)));
     k.row0 = block * kRows;
@@ -225,15 +225,16 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
   khd::grid_dependency_wait();
   khd::grid_dependents_may_launch();
 
-  const khp::Line line = khp::measure_line<kThreads, Cut>(P, scratch);
+  const khp::Line line = khp::lay_line<kThreads, Cut>(P, blockIdx.x, scratch);
   Walker walker{};
   walker.w = blockIdx.x;
-  if (static_cast<int>(blockIdx.x) < line.workers) {
-    walker.from = walker.at = khp::stretch(line, walker.w);
-    walker.until = khp::stretch(line, walker.w + 1);
-    khp::locate<kThreads, Cut>(P, walker.at, scratch, walker.b, walker.start);
+  if (walker.w < line.workers) {
+    walker.from = walker.at = line.stretch(walker.w);
+    walker.until = line.stretch(walker.w + 1);
+    walker.b = scratch.b;
+    walker.start = scratch.start;
   }
-  if (threadIdx.x == kThreads - 1) khp::note_split<Cut>(P, line, walker.w, walker.at, walker.b, walker.start);
+  if (threadIdx.x == kThreads - 1) khp::note_split<Cut>(P, line, walker.w, walker.b, walker.start);
   Work k;
 
   if (warp >= 8) {

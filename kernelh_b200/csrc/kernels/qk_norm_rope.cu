@@ -14,10 +14,15 @@
 // rotation exchanges nothing between lanes and the norm is the only reduction (log2(lanes) shuffles). A
 // row is read and written by the same lanes, read first: outputs may be the inputs themselves.
 //
+// A persistent grid whose blocks are dealt out to queries, keys (and values) by their share of the rows, so
+// that a block has one weight, kept in registers, and one set of weight-gradient sums. A block takes tiles of
+// tokens; its groups walk the tile's rows, the next row's loads in flight while one is worked on.
 // Angles: position * inv_freq in half turns, formed and reduced in 64 bits (a position of 10^6 times a
 // frequency of 1 has 20 bits before the point, fp32 would keep 4 after it), the remainder in [-1, 1]
-// rounded to fp32 for sincospif. They are worked out once per token by the whole block into shared memory
-// and shared by all its heads: 50 instructions each, which every head on its own would pay again.
+// rounded to fp32 for sincospif. They are worked out once per tile by the whole block into shared memory and
+// shared by all its heads: 50 instructions each, which every row on its own would pay again. Arithmetic on
+// pairs of values (fp32x2) and packed conversions: the kernels are bound by instructions before they are bound
+// by HBM (32768 tokens x 40 heads x 128 bf16: 370 instructions per row and warp, 202 us, before; MEASURE now).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -26,8 +31,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxPairs = 128;      // head_dim up to 256
-constexpr int kMaxTokensPerTile = 4;
+constexpr int kMaxAngles = 1024; // pairs x tokens of a tile
 
 // Rows of head_dim contiguous values: data + token * token_stride + head * head_stride (elements).
 struct HeadRows {
@@ -48,8 +52,9 @@ struct NormRopeParams {
   const int64_t *positions;
   int64_t tokens;
   int32_t q_heads, k_heads, head_dim, rotary_dim;
-  int32_t interleaved, lanes, tile_tokens;
+  int32_t lanes;          // of a row
   float eps;
+  int32_t blocks[3], tile[3]; // of queries, keys, values: blocks, and tokens of a tile
 };
 struct AppendParams {
   HeadRows v;
@@ -61,39 +66,223 @@ struct AppendParams {
 };
 struct BackwardParams {
   HeadRows dq_out, dk_out; // gradients that come in
-  float *partials;         // [gridDim.x][2][head_dim]
+  float *partials;         // [gridDim.x][head_dim]
 };
 struct WeightGradParams {
   const float *partials;
   float *dq_weight, *dk_weight; // either may be nullptr
-  int32_t blocks, head_dim;
+  int32_t blocks[2], head_dim;
 };
 
-template <typename T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+// Two values of 16 bits in a word.
+__device__ __forceinline__ float2 unpack(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float2 unpack(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t pack(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
 
-// kVec values of one access: 16, 8, 4 or 2 bytes.
+// The raw values of a lane's pairs: kSlots times two vectors of kVec values, of 16, 8, 4 or 2 bytes.
 template <int kBytes> struct Raw;
 template <> struct Raw<16> { using type = uint4; };
 template <> struct Raw<8> { using type = uint2; };
 template <> struct Raw<4> { using type = uint32_t; };
 template <> struct Raw<2> { using type = uint16_t; };
+template <typename T, int kVec, int kSlots> struct RawPairs {
+  using R = typename Raw<static_cast<int>(sizeof(T)) * kVec>::type;
+  R a[kSlots], b[kSlots];
+};
 
-template <typename T, int kVec> struct Vec {
-  using R = typename Raw<sizeof(T) * kVec>::type;
-  union {
-    R raw;
-    T v[kVec];
-  };
-  __device__ __forceinline__ Vec() {}
-  __device__ __forceinline__ void load(const T *p) { raw = __ldcs(reinterpret_cast<const R *>(p)); }
-  __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<R *>(p) = raw; }
+// A lane's pairs in fp32, two to a register pair.
+template <int kPairs> struct Pairs {
+  float2 a[kPairs / 2], b[kPairs / 2];
+};
+
+// How a kernel holds a row: kVec values per access; kSlots accesses per lane; kFull: every lane has all of them;
+// kInterleaved: pair j is (2j, 2j + 1), and the two vectors of a lane lie side by side.
+template <typename T_, int kVec_, int kSlots_, bool kFull_, bool kInterleaved_> struct Layout {
+  using T = T_;
+  static constexpr int kVec = kVec_, kSlots = kSlots_, kPairs = kVec * kSlots;
+  static constexpr bool kFull = kFull_, kInterleaved = kInterleaved_;
+  using RawT = RawPairs<T, kVec, kSlots>;
+  using Values = Pairs<kPairs>;
+
+  int first[kSlots], at_a[kSlots], at_b[kSlots]; // the slot's first pair, and where its vectors sit in a row
+  bool on[kSlots];
+  // Beyond the rotated part the remaining values are paired up the same way and pass through.
+  __device__ __forceinline__ Layout(const NormRopeParams &P, int lane) {
+    const int half = P.rotary_dim >> 1;
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      const int p = lane + s * P.lanes;
+      on[s] = kFull || 2 * p * kVec < P.head_dim;
+      first[s] = on[s] ? p * kVec : 0;
+      if (kInterleaved) {
+        at_a[s] = 2 * first[s];
+        at_b[s] = at_a[s] + kVec;
+      } else if (first[s] < half) {
+        at_a[s] = first[s];
+        at_b[s] = half + first[s];
+      } else {
+        at_a[s] = P.rotary_dim + (first[s] - half);
+        at_b[s] = at_a[s] + ((P.head_dim - P.rotary_dim) >> 1);
+      }
+    }
+  }
+  __device__ __forceinline__ void load(const T *row, RawT &v) const {
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+      if (on[s]) {
+        v.a[s] = __ldcs(reinterpret_cast<const typename RawT::R *>(row + at_a[s]));
+        v.b[s] = __ldcs(reinterpret_cast<const typename RawT::R *>(row + at_b[s]));
+      }
+  }
+  __device__ __forceinline__ void store(T *row, const RawT &v) const {
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+      if (on[s]) {
+        *reinterpret_cast<typename RawT::R *>(row + at_a[s]) = v.a[s];
+        *reinterpret_cast<typename RawT::R *>(row + at_b[s]) = v.b[s];
+      }
+  }
+  // Zeros for slots that are off.
+  __device__ __forceinline__ void widen(const RawT &v, bool mine, Values &x) const {
+    float a[kPairs], b[kPairs];
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      float y[2 * kVec]; // the values of a, then of b
+      if constexpr (sizeof(T) == 4) {
+        const float *pa = reinterpret_cast<const float *>(&v.a[s]), *pb = reinterpret_cast<const float *>(&v.b[s]);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) y[i] = pa[i], y[kVec + i] = pb[i];
+      } else if constexpr (kVec == 1) {
+        y[0] = unpack(v.a[s], T()).x;
+        y[1] = unpack(v.b[s], T()).x;
+      } else {
+        const uint32_t *pa = reinterpret_cast<const uint32_t *>(&v.a[s]), *pb = reinterpret_cast<const uint32_t *>(&v.b[s]);
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) {
+          const float2 p = unpack(pa[i], T()), q = unpack(pb[i], T());
+          y[2 * i] = p.x, y[2 * i + 1] = p.y, y[kVec + 2 * i] = q.x, y[kVec + 2 * i + 1] = q.y;
+        }
+      }
+      const bool keep = kFull ? mine : mine && on[s];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        a[s * kVec + i] = keep ? y[kInterleaved ? 2 * i : i] : 0.f;
+        b[s * kVec + i] = keep ? y[kInterleaved ? 2 * i + 1 : kVec + i] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs / 2; ++i) {
+      x.a[i] = make_float2(a[2 * i], a[2 * i + 1]);
+      x.b[i] = make_float2(b[2 * i], b[2 * i + 1]);
+    }
+  }
+  // The one rounding to the tensors' type.
+  __device__ __forceinline__ void narrow(const Values &x, RawT &v) const {
+    float a[kPairs], b[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs / 2; ++i) {
+      a[2 * i] = x.a[i].x, a[2 * i + 1] = x.a[i].y;
+      b[2 * i] = x.b[i].x, b[2 * i + 1] = x.b[i].y;
+    }
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      float y[2 * kVec];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        y[kInterleaved ? 2 * i : i] = a[s * kVec + i];
+        y[kInterleaved ? 2 * i + 1 : kVec + i] = b[s * kVec + i];
+      }
+      if constexpr (sizeof(T) == 4) {
+        float *pa = reinterpret_cast<float *>(&v.a[s]), *pb = reinterpret_cast<float *>(&v.b[s]);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) pa[i] = y[i], pb[i] = y[kVec + i];
+      } else if constexpr (kVec == 1) {
+        v.a[s] = static_cast<uint16_t>(pack(y[0], 0.f, T()));
+        v.b[s] = static_cast<uint16_t>(pack(y[1], 0.f, T()));
+      } else {
+        uint32_t *pa = reinterpret_cast<uint32_t *>(&v.a[s]), *pb = reinterpret_cast<uint32_t *>(&v.b[s]);
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) pa[i] = pack(y[2 * i], y[2 * i + 1], T()), pb[i] = pack(y[kVec + 2 * i], y[kVec + 2 * i + 1], T());
+      }
+    }
+  }
+  // Values of a head_dim vector (a weight; a null one is all ones) that belong to this lane's pairs.
+  __device__ __forceinline__ void weights(const float *w, Values &x) const {
+    float a[kPairs], b[kPairs];
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        a[s * kVec + i] = w != nullptr && on[s] ? __ldg(w + at(s, i, false)) : 1.f;
+        b[s * kVec + i] = w != nullptr && on[s] ? __ldg(w + at(s, i, true)) : 1.f;
+      }
+#pragma unroll
+    for (int i = 0; i < kPairs / 2; ++i) {
+      x.a[i] = make_float2(a[2 * i], a[2 * i + 1]);
+      x.b[i] = make_float2(b[2 * i], b[2 * i + 1]);
+    }
+  }
+  __device__ __forceinline__ int at(int s, int i, bool second) const {
+    return kInterleaved ? at_a[s] + 2 * i + second : (second ? at_b[s] : at_a[s]) + i;
+  }
+  // cos and sin of this lane's pairs out of a token's table.
+  __device__ __forceinline__ void angles(const float *cs, const float *sn, float2 (&c)[kPairs / 2], float2 (&s)[kPairs / 2]) const {
+    float fc[kPairs], fs[kPairs];
+#pragma unroll
+    for (int x = 0; x < kSlots; ++x) {
+      if constexpr (kVec % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < kVec; i += 4) {
+          *reinterpret_cast<float4 *>(&fc[x * kVec + i]) = *reinterpret_cast<const float4 *>(cs + first[x] + i);
+          *reinterpret_cast<float4 *>(&fs[x * kVec + i]) = *reinterpret_cast<const float4 *>(sn + first[x] + i);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          fc[x * kVec + i] = cs[first[x] + i];
+          fs[x * kVec + i] = sn[first[x] + i];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs / 2; ++i) {
+      c[i] = make_float2(fc[2 * i], fc[2 * i + 1]);
+      s[i] = make_float2(fs[2 * i], fs[2 * i + 1]);
+    }
+  }
+  // Turns the pairs by their angles (`sign` -1: back). Pairs from `half` on stay exactly as they are.
+  template <int sign> __device__ __forceinline__ void rotate(Values &x, const float2 (&c)[kPairs / 2], const float2 (&s)[kPairs / 2], int half) const {
+    bool all = true;
+#pragma unroll
+    for (int y = 0; y < kSlots; ++y) all = all && first[y] + kVec <= half;
+#pragma unroll
+    for (int i = 0; i < kPairs / 2; ++i) {
+      const float2 p = x.a[i], q = x.b[i];
+      const float2 qs = __fmul2_rn(q, s[i]), ps = __fmul2_rn(p, s[i]);
+      float2 a, b;
+      if (sign > 0) {
+        a = make_float2(fmaf(p.x, c[i].x, -qs.x), fmaf(p.y, c[i].y, -qs.y));
+        b = __ffma2_rn(q, c[i], ps);
+      } else {
+        a = __ffma2_rn(p, c[i], qs);
+        b = make_float2(fmaf(q.x, c[i].x, -ps.x), fmaf(q.y, c[i].y, -ps.y));
+      }
+      if (!all) {
+        const bool x0 = first[2 * i / kVec] + 2 * i % kVec < half, x1 = first[(2 * i + 1) / kVec] + (2 * i + 1) % kVec < half;
+        a = make_float2(x0 ? a.x : p.x, x1 ? a.y : p.y);
+        b = make_float2(x0 ? b.x : q.x, x1 ? b.y : q.y);
+      }
+      x.a[i] = a;
+      x.b[i] = b;
+    }
+  }
 };
 
 // The sum over the row's lanes (a power of two, aligned inside the warp), the same bits in every lane.
@@ -103,410 +292,286 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
     if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-
-// Where the two vectors of pair-vector `p` (pairs p * kVec ..) sit in a row. Beyond the rotated part the
-// remaining values are paired up the same way and pass through.
-template <int kVec> __device__ __forceinline__ void pair_offsets(int p, const NormRopeParams &P, int &a, int &b) {
-  if (P.interleaved) {
-    a = 2 * p * kVec;
-    b = a + kVec;
-    return;
+template <int kPairs> __device__ __forceinline__ float dot(const Pairs<kPairs> &x, const Pairs<kPairs> &y) {
+  float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < kPairs / 2; ++i) {
+    s = __ffma2_rn(x.a[i], y.a[i], s);
+    s = __ffma2_rn(x.b[i], y.b[i], s);
   }
-  const int half = P.rotary_dim >> 1, first = p * kVec;
-  if (first < half) {
-    a = first;
-    b = half + first;
-  } else {
-    a = P.rotary_dim + (first - half);
-    b = a + ((P.head_dim - P.rotary_dim) >> 1);
-  }
+  return s.x + s.y;
 }
 
-// cos and sin of every pair of the tile's tokens, (1, 0) past the rotated part. The sine's sign is the caller's.
-__device__ __forceinline__ void fill_angles(const NormRopeParams &P, int64_t token0, float (*cs)[kMaxPairs], float (*sn)[kMaxPairs]) {
+// cos and sin of every pair of the tile's tokens, (1, 0) past the rotated part.
+__device__ __forceinline__ void fill_angles(const NormRopeParams &P, int64_t token0, int tokens, float *cs, float *sn) {
   const int pairs = P.head_dim >> 1, half = P.rotary_dim >> 1;
-  for (int i = threadIdx.x; i < P.tile_tokens * pairs; i += kThreads) {
+  for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
     const int t = i / pairs, j = i - t * pairs;
     float c = 1.f, s = 0.f;
-    if (j < half && token0 + t < P.tokens) {
+    if (j < half) {
       const double turns = static_cast<double>(P.positions[token0 + t]) * static_cast<double>(P.inv_freq[j]) * 0.31830988618379067154;
       sincospif(static_cast<float>(turns - 2.0 * rint(0.5 * turns)), &s, &c);
     }
-    cs[t][j] = c;
-    sn[t][j] = s;
+    cs[i] = c;
+    sn[i] = s;
   }
 }
 
-// n = x r w for one row: `a` and `b` hold the raw pair vectors on entry, xa / xb their values x and the result is r.
-template <typename T, int kVec, int kSlots>
-__device__ __forceinline__ float row_rms(const Vec<T, kVec> (&a)[kSlots], const Vec<T, kVec> (&b)[kSlots], const bool (&on)[kSlots],
-                                         const NormRopeParams &P, float (&xa)[kSlots][kVec], float (&xb)[kSlots][kVec]) {
-  float sum = 0.f;
-#pragma unroll
-  for (int s = 0; s < kSlots; ++s)
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      xa[s][i] = on[s] ? to_float(a[s].v[i]) : 0.f;
-      xb[s][i] = on[s] ? to_float(b[s].v[i]) : 0.f;
-      sum = fmaf(xa[s][i], xa[s][i], sum);
-      sum = fmaf(xb[s][i], xb[s][i], sum);
-    }
-  return rsqrtf(group_sum(sum, P.lanes) / static_cast<float>(P.head_dim) + P.eps);
-}
-
-// (a, b) turned by (c, s) pairwise, in place. Interleaved pairs lie in one vector: the i-th pair of the
-// 2 kVec contiguous values is (value 2i, value 2i + 1). Pairs from `half` on stay as they are.
-template <int kVec>
-__device__ __forceinline__ void rotate(float (&a)[kVec], float (&b)[kVec], const float (&c)[kVec], const float (&s)[kVec], int first,
-                                       int half, bool interleaved) {
-  if (!interleaved) {
-    if (first >= half) return;
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const float x = a[i], y = b[i];
-      a[i] = x * c[i] - y * s[i];
-      b[i] = x * s[i] + y * c[i];
-    }
-    return;
+// A block's part of the work: which rows, and of them which tiles. Its groups of lanes walk the rows of a tile:
+// group, group + groups, ...; a row is (token of the tile, head).
+struct Share {
+  int kind, heads, tile, block, blocks; // kind 0 queries, 1 keys, 2 values
+  int groups, group, lane;
+  int token_step, head_step, token_first, head_first;
+  __device__ __forceinline__ Share(const NormRopeParams &P) {
+    block = blockIdx.x;
+    kind = 0;
+    while (block >= P.blocks[kind]) block -= P.blocks[kind++];
+    heads = kind == 0 ? P.q_heads : P.k_heads;
+    tile = P.tile[kind];
+    blocks = P.blocks[kind];
+    groups = kThreads / P.lanes;
+    group = threadIdx.x / P.lanes;
+    lane = threadIdx.x % P.lanes;
+    token_step = groups / heads;
+    head_step = groups % heads;
+    token_first = group / heads;
+    head_first = group % heads;
   }
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    float &ra = 2 * i < kVec ? a[(2 * i) % kVec] : b[(2 * i) % kVec];
-    float &rb = 2 * i + 1 < kVec ? a[(2 * i + 1) % kVec] : b[(2 * i + 1) % kVec];
-    if (first + i < half) {
-      const float x = ra, y = rb;
-      ra = x * c[i] - y * s[i];
-      rb = x * s[i] + y * c[i];
-    }
-  }
-}
-
-template <typename T, int kVec, int kSlots>
-__device__ __forceinline__ void load_row(Vec<T, kVec> (&a)[kSlots], Vec<T, kVec> (&b)[kSlots], const HeadRows &rows, int64_t token,
-                                         int head, const int (&at_a)[kSlots], const int (&at_b)[kSlots], const bool (&on)[kSlots]) {
-  const T *p = reinterpret_cast<const T *>(rows.data) + token * rows.token_stride + head * rows.head_stride;
-#pragma unroll
-  for (int s = 0; s < kSlots; ++s)
-    if (on[s]) {
-      a[s].load(p + at_a[s]);
-      b[s].load(p + at_b[s]);
-    }
-}
-
-// The geometry of a lane: kSlots pair vectors `lane + s * lanes`, of which those inside the row are on.
-template <int kVec, int kSlots> struct LaneMap {
-  int first[kSlots], at_a[kSlots], at_b[kSlots];
-  bool on[kSlots];
-  __device__ __forceinline__ LaneMap(const NormRopeParams &P, int lane) {
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s) {
-      const int p = lane + s * P.lanes;
-      on[s] = 2 * p * kVec < P.head_dim;
-      first[s] = on[s] ? p * kVec : 0;
-      pair_offsets<kVec>(on[s] ? p : 0, P, at_a[s], at_b[s]);
+  __device__ __forceinline__ void next(int &token, int &head) const {
+    token += token_step;
+    head += head_step;
+    if (head >= heads) {
+      head -= heads;
+      ++token;
     }
   }
 };
-
-// Weights of the lane's values: wa[s][i] belongs to offset at_a[s] + i. A null weight is all ones.
-template <int kVec, int kSlots>
-__device__ __forceinline__ void load_weights(const float *w, const LaneMap<kVec, kSlots> &m, float (&wa)[kSlots][kVec], float (&wb)[kSlots][kVec]) {
-#pragma unroll
-  for (int s = 0; s < kSlots; ++s)
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      wa[s][i] = w != nullptr && m.on[s] ? __ldg(w + m.at_a[s] + i) : 1.f;
-      wb[s][i] = w != nullptr && m.on[s] ? __ldg(w + m.at_b[s] + i) : 1.f;
-    }
+template <typename T> __device__ __forceinline__ T *row_of(const HeadRows &rows, int64_t token, int head) {
+  return reinterpret_cast<T *>(rows.data) + token * rows.token_stride + head * rows.head_stride;
 }
 
-// Forward. A block takes tile_tokens tokens; its lane groups are dealt out to the tokens evenly and a group
-// walks the heads of its token (queries, keys, and the values when they are appended) with its cosines in
-// registers, the next row's loads in flight while it works on the current one.
-template <typename T, int kVec, int kSlots, bool kAppend>
-__device__ __forceinline__ void forward_body(const NormRopeParams &P, const AppendParams &A) {
-  __shared__ float s_cos[kMaxTokensPerTile][kMaxPairs], s_sin[kMaxTokensPerTile][kMaxPairs];
-  const int groups_per_token = kThreads / P.lanes / P.tile_tokens;
-  const int group = threadIdx.x / P.lanes, lane = threadIdx.x % P.lanes;
-  const int t = group / groups_per_token;
-  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * P.tile_tokens;
-  const int64_t token = token0 + t;
-  const int heads = P.q_heads + P.k_heads + (kAppend ? P.k_heads : 0);
-  const LaneMap<kVec, kSlots> m(P, lane);
+template <typename L, bool kAppend> __device__ __forceinline__ void forward_body(const NormRopeParams &P, const AppendParams &A) {
+  using T = typename L::T;
+  __shared__ __align__(16) float s_cos[2][kMaxAngles], s_sin[2][kMaxAngles];
+  __shared__ int64_t s_place[2][kAppend ? kMaxAngles : 1]; // where the token's rows go in the cache (INT64_MIN: nowhere)
+  const Share me(P);
+  const L lay(P, me.lane);
+  const int half = P.rotary_dim >> 1, pairs = P.head_dim >> 1;
+  const float scale = 1.f / static_cast<float>(P.head_dim);
   khd::grid_dependency_wait();
   khd::grid_dependents_may_launch();
-
-  const bool live = token < P.tokens;
-  Vec<T, kVec> a[kSlots], b[kSlots];
-  const auto fetch = [&](int head) {
-    if (head < P.q_heads) load_row<T, kVec, kSlots>(a, b, P.q, token, head, m.at_a, m.at_b, m.on);
-    else if (head < P.q_heads + P.k_heads) load_row<T, kVec, kSlots>(a, b, P.k, token, head - P.q_heads, m.at_a, m.at_b, m.on);
-    else if (kAppend) load_row<T, kVec, kSlots>(a, b, A.v, token, head - P.q_heads - P.k_heads, m.at_a, m.at_b, m.on);
-  };
-  int head = group % groups_per_token;
-  if (live && head < heads) fetch(head);
-
-  int64_t slot = -1, page = 0;
-  int in_page = 0;
-  if (kAppend && live) {
-    slot = __ldg(A.slots + token);
-    if (slot < -1 || slot >= A.num_slots) { // nothing is stored for this token, and the host is told
-      if (lane == 0) khd::report_status(A.status, khd::kStatusBadSlot, static_cast<uint32_t>(token));
-      slot = -1;
-    }
-    if (slot >= 0) {
-      page = slot / A.page_size;
-      in_page = static_cast<int>(slot - page * A.page_size);
-    }
-  }
-  fill_angles(P, token0, s_cos, s_sin);
-  __syncthreads();
-  float c[kSlots][kVec], s[kSlots][kVec];
-#pragma unroll
-  for (int x = 0; x < kSlots; ++x)
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      c[x][i] = s_cos[t][m.first[x] + i];
-      s[x][i] = s_sin[t][m.first[x] + i];
-    }
-  float wa[kSlots][kVec], wb[kSlots][kVec];
-  int have = -1; // whose weights are in the registers: 0 queries, 1 keys
-  const int half = P.rotary_dim >> 1;
-  // every lane of a warp walks the same number of rows, so that the shuffles are always complete
-  for (int h0 = 0; h0 < heads; h0 += groups_per_token, head += groups_per_token) {
-    const bool mine = live && head < heads;
-    const int kind = head < P.q_heads ? 0 : (head < P.q_heads + P.k_heads ? 1 : 2);
-    Vec<T, kVec> oa[kSlots], ob[kSlots];
-    float xa[kSlots][kVec], xb[kSlots][kVec];
-    bool used[kSlots];
-#pragma unroll
-    for (int x = 0; x < kSlots; ++x) {
-      used[x] = mine && m.on[x];
-      oa[x] = a[x];
-      ob[x] = b[x];
-    }
-    if (live && head + groups_per_token < heads) fetch(head + groups_per_token);
-    const float r = row_rms<T, kVec, kSlots>(oa, ob, used, P, xa, xb);
-    if (!mine) continue;
-    if (kind < 2) {
-      if (kind != have) {
-        load_weights<kVec, kSlots>(kind == 0 ? P.q_weight : P.k_weight, m, wa, wb);
-        have = kind;
-      }
-#pragma unroll
-      for (int x = 0; x < kSlots; ++x) {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          xa[x][i] = xa[x][i] * r * wa[x][i];
-          xb[x][i] = xb[x][i] * r * wb[x][i];
-        }
-        rotate<kVec>(xa[x], xb[x], c[x], s[x], m.first[x], half, P.interleaved != 0);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          oa[x].v[i] = from_float<T>(xa[x][i]); // the one rounding to the tensors' type
-          ob[x].v[i] = from_float<T>(xb[x][i]);
-        }
-      }
-    }
-    T *out;
-    if (kind == 0) {
-      out = reinterpret_cast<T *>(P.q_out.data) + token * P.q_out.token_stride + head * P.q_out.head_stride;
-    } else if (!kAppend) {
-      out = reinterpret_cast<T *>(P.k_out.data) + token * P.k_out.token_stride + (head - P.q_heads) * P.k_out.head_stride;
-    } else {
-      if (slot < 0) continue;
-      const PagedRows &cache = kind == 1 ? A.k_cache : A.v_cache;
-      const int at = head - P.q_heads - (kind == 2 ? P.k_heads : 0);
-      out = reinterpret_cast<T *>(cache.data) + page * cache.page_stride + in_page * cache.slot_stride + at * cache.head_stride;
-    }
-#pragma unroll
-    for (int x = 0; x < kSlots; ++x)
-      if (m.on[x]) {
-        oa[x].store(out + m.at_a[x]);
-        ob[x].store(out + m.at_b[x]);
-      }
-  }
-}
-
-// Backward. A persistent grid: a block walks the tiles blockIdx.x, + gridDim.x, ... and every lane keeps the
-// weight gradients of its own values, for queries and for keys, in fp32 registers over all its rows. At the
-// end the block adds its groups' sums in a fixed order into one row of `partials`, which
-// qk_norm_weight_grad adds up over the blocks, again in a fixed order: no atomics, the same bits every time.
-template <typename T, int kVec, int kSlots> __device__ __forceinline__ void backward_body(const NormRopeParams &P, const BackwardParams &B) {
-  __shared__ float s_cos[2][kMaxTokensPerTile][kMaxPairs], s_sin[2][kMaxTokensPerTile][kMaxPairs];
-  __shared__ float s_sum[kThreads / 32][2][2 * kMaxPairs];
-  const int groups_per_token = kThreads / P.lanes / P.tile_tokens;
-  const int group = threadIdx.x / P.lanes, lane = threadIdx.x % P.lanes;
-  const int t = group / groups_per_token;
-  const int heads = P.q_heads + P.k_heads;
-  const int half = P.rotary_dim >> 1;
-  const LaneMap<kVec, kSlots> m(P, lane);
-  float wsum[2][2][kSlots][kVec];
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int x = 0; x < kSlots; ++x)
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) wsum[k][0][x][i] = wsum[k][1][x][i] = 0.f;
-  khd::grid_dependency_wait();
-  khd::grid_dependents_may_launch();
-  const int64_t tiles = (P.tokens + P.tile_tokens - 1) / P.tile_tokens;
+  const HeadRows in = me.kind == 0 ? P.q : me.kind == 1 ? P.k : A.v;
+  const HeadRows out = me.kind == 0 ? P.q_out : P.k_out;
+  const PagedRows cache = me.kind == 1 ? A.k_cache : A.v_cache;
+  typename L::Values w;
+  lay.weights(me.kind == 0 ? P.q_weight : me.kind == 1 ? P.k_weight : nullptr, w);
+  const int64_t tiles = (P.tokens + me.tile - 1) / me.tile;
   int buffer = 0;
-  float wa[kSlots][kVec], wb[kSlots][kVec];
-  int have = -1;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, buffer ^= 1) {
-    const int64_t token0 = tile * P.tile_tokens, token = token0 + t;
-    const bool live = token < P.tokens;
-    Vec<T, kVec> a[kSlots], b[kSlots], da[kSlots], db[kSlots];
-    const auto fetch = [&](int head) {
-      const bool is_q = head < P.q_heads;
-      const int at = is_q ? head : head - P.q_heads;
-      load_row<T, kVec, kSlots>(a, b, is_q ? P.q : P.k, token, at, m.at_a, m.at_b, m.on);
-      load_row<T, kVec, kSlots>(da, db, is_q ? B.dq_out : B.dk_out, token, at, m.at_a, m.at_b, m.on);
-    };
-    int head = group % groups_per_token;
-    if (live && head < heads) fetch(head);
-    fill_angles(P, token0, s_cos[buffer], s_sin[buffer]);
-    __syncthreads(); // the other buffer's readers are past this barrier's predecessor before it is refilled
-    float c[kSlots][kVec], s[kSlots][kVec];
-#pragma unroll
-    for (int x = 0; x < kSlots; ++x)
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        c[x][i] = s_cos[buffer][t][m.first[x] + i];
-        s[x][i] = -s_sin[buffer][t][m.first[x] + i]; // the inverse rotation
-      }
-    for (int h0 = 0; h0 < heads; h0 += groups_per_token, head += groups_per_token) {
-      const bool mine = live && head < heads;
-      const bool is_q = head < P.q_heads;
-      float xa[kSlots][kVec], xb[kSlots][kVec], ga[kSlots][kVec], gb[kSlots][kVec];
-      bool used[kSlots];
-#pragma unroll
-      for (int x = 0; x < kSlots; ++x) {
-        used[x] = mine && m.on[x];
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          ga[x][i] = used[x] ? to_float(da[x].v[i]) : 0.f;
-          gb[x][i] = used[x] ? to_float(db[x].v[i]) : 0.f;
+  for (int64_t tile = me.block; tile < tiles; tile += me.blocks, buffer ^= 1) {
+    const int64_t token0 = tile * me.tile;
+    const int tokens = static_cast<int>(min(static_cast<int64_t>(me.tile), P.tokens - token0)), rows = tokens * me.heads;
+    typename L::RawT raw;
+    int t = me.token_first, h = me.head_first;
+    if (me.group < rows) lay.load(row_of<T>(in, token0 + t, h), raw);
+    if (kAppend && me.kind > 0) {
+      for (int i = threadIdx.x; i < tokens; i += kThreads) {
+        const int64_t slot = A.slots[token0 + i];
+        int64_t place = INT64_MIN;
+        if (slot >= 0 && slot < A.num_slots) {
+          const int64_t page = slot < (int64_t{1} << 31) ? static_cast<uint32_t>(slot) / static_cast<uint32_t>(A.page_size) : slot / A.page_size;
+          place = page * cache.page_stride + (slot - page * A.page_size) * cache.slot_stride;
+        } else if (slot != -1) { // nothing is stored for this token, and the host is told
+          khd::report_status(A.status, khd::kStatusBadSlot, static_cast<uint32_t>(token0 + i));
         }
+        s_place[buffer][i] = place;
       }
-      const float r = row_rms<T, kVec, kSlots>(a, b, used, P, xa, xb);
-      if (live && head + groups_per_token < heads) fetch(head + groups_per_token);
-      if (mine && have != (is_q ? 0 : 1)) {
-        have = is_q ? 0 : 1;
-        load_weights<kVec, kSlots>(is_q ? P.q_weight : P.k_weight, m, wa, wb);
-      }
-      float dot = 0.f; // sum of g w u
+    }
+    if (me.kind < 2) fill_angles(P, token0, tokens, s_cos[buffer], s_sin[buffer]);
+    __syncthreads(); // the other buffers' readers passed the barrier before this one
+    // every lane of a warp makes the same number of turns, so that the shuffles are always complete
+    for (int r0 = 0; r0 < rows; r0 += me.groups) {
+      const bool mine = r0 + me.group < rows;
+      typename L::RawT cur = raw;
+      int t_next = t, h_next = h;
+      me.next(t_next, h_next);
+      if (r0 + me.groups + me.group < rows) lay.load(row_of<T>(in, token0 + t_next, h_next), raw);
+      if (!kAppend || me.kind < 2) {
+        typename L::Values x;
+        lay.widen(cur, mine, x);
+        const float r = rsqrtf(fmaf(group_sum(dot(x, x), P.lanes), scale, P.eps));
+        if (mine) {
+          float2 c[L::kPairs / 2], s[L::kPairs / 2];
+          lay.angles(s_cos[buffer] + t * pairs, s_sin[buffer] + t * pairs, c, s);
+          const float2 r2 = make_float2(r, r);
 #pragma unroll
-      for (int x = 0; x < kSlots; ++x) {
-        rotate<kVec>(ga[x], gb[x], c[x], s[x], m.first[x], half, P.interleaved != 0);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          xa[x][i] *= r; // u
-          xb[x][i] *= r;
-          const float va = ga[x][i] * xa[x][i], vb = gb[x][i] * xb[x][i];
-          if (used[x]) {
-            if (is_q) {
-              wsum[0][0][x][i] += va;
-              wsum[0][1][x][i] += vb;
-            } else {
-              wsum[1][0][x][i] += va;
-              wsum[1][1][x][i] += vb;
-            }
-            dot = fmaf(va, wa[x][i], dot);
-            dot = fmaf(vb, wb[x][i], dot);
+          for (int i = 0; i < L::kPairs / 2; ++i) {
+            x.a[i] = __fmul2_rn(__fmul2_rn(x.a[i], r2), w.a[i]);
+            x.b[i] = __fmul2_rn(__fmul2_rn(x.b[i], r2), w.b[i]);
           }
+          lay.template rotate<1>(x, c, s, half);
+          lay.narrow(x, cur);
         }
       }
-      const float mean = group_sum(dot, P.lanes) / static_cast<float>(P.head_dim);
-      if (!mine) continue;
-      const HeadRows &rows = is_q ? P.q_out : P.k_out;
-      T *out = reinterpret_cast<T *>(rows.data) + token * rows.token_stride + (is_q ? head : head - P.q_heads) * rows.head_stride;
-#pragma unroll
-      for (int x = 0; x < kSlots; ++x)
-        if (m.on[x]) {
-          Vec<T, kVec> oa, ob;
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            oa.v[i] = from_float<T>(r * (ga[x][i] * wa[x][i] - xa[x][i] * mean));
-            ob.v[i] = from_float<T>(r * (gb[x][i] * wb[x][i] - xb[x][i] * mean));
-          }
-          oa.store(out + m.at_a[x]);
-          ob.store(out + m.at_b[x]);
+      if (mine) {
+        if (!kAppend || me.kind == 0) {
+          lay.store(row_of<T>(out, token0 + t, h), cur);
+        } else if (const int64_t place = s_place[buffer][t]; place != INT64_MIN) {
+          lay.store(reinterpret_cast<T *>(cache.data) + place + h * cache.head_stride, cur);
         }
+      }
+      t = t_next;
+      h = h_next;
+    }
+  }
+}
+
+// Backward. Every lane keeps the weight gradients of its own values in fp32 registers over all its rows. At the end
+// the block adds its groups' sums in a fixed order into one row of `partials`, which qk_norm_weight_grad adds up
+// over the blocks, again in a fixed order: no atomics, the same bits every time.
+template <typename L> __device__ __forceinline__ void backward_body(const NormRopeParams &P, const BackwardParams &B) {
+  using T = typename L::T;
+  __shared__ __align__(16) float s_cos[2][kMaxAngles], s_sin[2][kMaxAngles];
+  __shared__ float s_sum[kThreads / 32][256];
+  const Share me(P);
+  const L lay(P, me.lane);
+  const int half = P.rotary_dim >> 1, pairs = P.head_dim >> 1;
+  const float scale = 1.f / static_cast<float>(P.head_dim);
+  khd::grid_dependency_wait();
+  khd::grid_dependents_may_launch();
+  const HeadRows in = me.kind == 0 ? P.q : P.k, grad = me.kind == 0 ? B.dq_out : B.dk_out, out = me.kind == 0 ? P.q_out : P.k_out;
+  typename L::Values w, sum;
+  lay.weights(me.kind == 0 ? P.q_weight : P.k_weight, w);
+#pragma unroll
+  for (int i = 0; i < L::kPairs / 2; ++i) sum.a[i] = sum.b[i] = make_float2(0.f, 0.f);
+  const int64_t tiles = (P.tokens + me.tile - 1) / me.tile;
+  int buffer = 0;
+  for (int64_t tile = me.block; tile < tiles; tile += me.blocks, buffer ^= 1) {
+    const int64_t token0 = tile * me.tile;
+    const int tokens = static_cast<int>(min(static_cast<int64_t>(me.tile), P.tokens - token0)), rows = tokens * me.heads;
+    typename L::RawT raw, draw;
+    int t = me.token_first, h = me.head_first;
+    if (me.group < rows) {
+      lay.load(row_of<T>(in, token0 + t, h), raw);
+      lay.load(row_of<T>(grad, token0 + t, h), draw);
+    }
+    fill_angles(P, token0, tokens, s_cos[buffer], s_sin[buffer]);
+    __syncthreads(); // the other buffer's readers passed the barrier before this one
+    for (int r0 = 0; r0 < rows; r0 += me.groups) {
+      const bool mine = r0 + me.group < rows;
+      typename L::Values u, g;
+      lay.widen(raw, mine, u);
+      lay.widen(draw, mine, g);
+      int t_next = t, h_next = h;
+      me.next(t_next, h_next);
+      if (r0 + me.groups + me.group < rows) {
+        lay.load(row_of<T>(in, token0 + t_next, h_next), raw);
+        lay.load(row_of<T>(grad, token0 + t_next, h_next), draw);
+      }
+      const float r = rsqrtf(fmaf(group_sum(dot(u, u), P.lanes), scale, P.eps));
+      const float2 r2 = make_float2(r, r);
+      float2 c[L::kPairs / 2], s[L::kPairs / 2];
+      const int at = (mine ? t : 0) * pairs;
+      lay.angles(s_cos[buffer] + at, s_sin[buffer] + at, c, s);
+      lay.template rotate<-1>(g, c, s, half);
+#pragma unroll
+      for (int i = 0; i < L::kPairs / 2; ++i) {
+        u.a[i] = __fmul2_rn(u.a[i], r2);
+        u.b[i] = __fmul2_rn(u.b[i], r2);
+        sum.a[i] = __ffma2_rn(g.a[i], u.a[i], sum.a[i]);
+        sum.b[i] = __ffma2_rn(g.b[i], u.b[i], sum.b[i]);
+        g.a[i] = __fmul2_rn(g.a[i], w.a[i]);
+        g.b[i] = __fmul2_rn(g.b[i], w.b[i]);
+      }
+      const float mean = group_sum(dot(g, u), P.lanes) * scale;
+      if (mine) {
+        const float2 m2 = make_float2(-mean, -mean);
+#pragma unroll
+        for (int i = 0; i < L::kPairs / 2; ++i) {
+          g.a[i] = __fmul2_rn(__ffma2_rn(u.a[i], m2, g.a[i]), r2);
+          g.b[i] = __fmul2_rn(__ffma2_rn(u.b[i], m2, g.b[i]), r2);
+        }
+        typename L::RawT res;
+        lay.narrow(g, res);
+        lay.store(row_of<T>(out, token0 + t, h), res);
+      }
+      t = t_next;
+      h = h_next;
     }
   }
   // groups of a warp first (shuffles over the lanes that hold the same values), then the eight warps
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int x = 0; x < kSlots; ++x)
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        float va = wsum[k][0][x][i], vb = wsum[k][1][x][i];
-        for (int o = P.lanes; o < 32; o <<= 1) {
-          va += __shfl_xor_sync(0xffffffffu, va, o);
-          vb += __shfl_xor_sync(0xffffffffu, vb, o);
-        }
-        if ((threadIdx.x & 31) < P.lanes && m.on[x]) {
-          s_sum[threadIdx.x >> 5][k][m.at_a[x] + i] = va;
-          s_sum[threadIdx.x >> 5][k][m.at_b[x] + i] = vb;
-        }
-      }
+  for (int i = 0; i < L::kPairs; ++i) {
+    float a = i & 1 ? sum.a[i / 2].y : sum.a[i / 2].x, b = i & 1 ? sum.b[i / 2].y : sum.b[i / 2].x;
+    for (int o = P.lanes; o < 32; o <<= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    if ((threadIdx.x & 31) < P.lanes && lay.on[i / L::kVec]) {
+      s_sum[threadIdx.x >> 5][lay.at(i / L::kVec, i % L::kVec, false)] = a;
+      s_sum[threadIdx.x >> 5][lay.at(i / L::kVec, i % L::kVec, true)] = b;
+    }
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * P.head_dim; i += kThreads) {
-    const int k = i / P.head_dim, at = i - k * P.head_dim;
+  for (int i = threadIdx.x; i < P.head_dim; i += kThreads) {
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) v += s_sum[w][k][at];
-    B.partials[(static_cast<int64_t>(blockIdx.x) * 2 + k) * P.head_dim + at] = v;
+    for (int x = 0; x < kThreads / 32; ++x) v += s_sum[x][i];
+    B.partials[static_cast<int64_t>(blockIdx.x) * P.head_dim + i] = v;
   }
 }
 
 } // namespace
 
-#define KH_NORM_ROPE(suffix, T, vec, slots)                                                                              \
-  extern "C" __global__ void __launch_bounds__(kThreads)                                                                \
+#define KH_NORM_ROPE_PAIRING(suffix, T, vec, slots, full, pairing)                                                      \
+  extern "C" __global__ void __launch_bounds__(kThreads, 3)                                                             \
   qk_norm_rope_##suffix(const __grid_constant__ NormRopeParams P) {                                                     \
-    forward_body<T, vec, slots, false>(P, AppendParams{});                                                              \
+    forward_body<Layout<T, vec, slots, full, pairing>, false>(P, AppendParams{});                                       \
   }                                                                                                                     \
-  extern "C" __global__ void __launch_bounds__(kThreads)                                                                \
+  extern "C" __global__ void __launch_bounds__(kThreads, 3)                                                             \
   qk_norm_rope_append_##suffix(const __grid_constant__ NormRopeParams P, const __grid_constant__ AppendParams A) {      \
-    forward_body<T, vec, slots, true>(P, A);                                                                            \
+    forward_body<Layout<T, vec, slots, full, pairing>, true>(P, A);                                                     \
   }                                                                                                                     \
-  extern "C" __global__ void __launch_bounds__(kThreads)                                                                \
+  extern "C" __global__ void __launch_bounds__(kThreads, 2)                                                             \
   qk_norm_rope_backward_##suffix(const __grid_constant__ NormRopeParams P, const __grid_constant__ BackwardParams B) {  \
-    backward_body<T, vec, slots>(P, B);                                                                                 \
+    backward_body<Layout<T, vec, slots, full, pairing>>(P, B);                                                          \
   }
+#define KH_NORM_ROPE(suffix, T, vec, slots, full)                \
+  KH_NORM_ROPE_PAIRING(suffix##_halves, T, vec, slots, full, false) \
+  KH_NORM_ROPE_PAIRING(suffix##_inter, T, vec, slots, full, true)
 
-// 16-byte vectors; 8-byte ones for halves of a rotation, or addresses, that 16 bytes do not divide; single
-// values (four pairs per lane, 32 lanes) for everything else.
-KH_NORM_ROPE(f32_v4, float, 4, 1)
-KH_NORM_ROPE(f32_v2, float, 2, 1)
-KH_NORM_ROPE(f32_v1, float, 1, 4)
-KH_NORM_ROPE(bf16_v8, __nv_bfloat16, 8, 1)
-KH_NORM_ROPE(bf16_v4, __nv_bfloat16, 4, 1)
-KH_NORM_ROPE(bf16_v1, __nv_bfloat16, 1, 4)
-KH_NORM_ROPE(f16_v8, __half, 8, 1)
-KH_NORM_ROPE(f16_v4, __half, 4, 1)
-KH_NORM_ROPE(f16_v1, __half, 1, 4)
+// 16-byte vectors (full: and no idle lane); 8-byte ones for halves of a rotation, or addresses, that 16 bytes do not
+// divide; single values (four pairs per lane) for everything else.
+KH_NORM_ROPE(f32_v4_full, float, 4, 1, true)
+KH_NORM_ROPE(f32_v4, float, 4, 1, false)
+KH_NORM_ROPE(f32_v2, float, 2, 1, false)
+KH_NORM_ROPE(f32_v1, float, 1, 4, false)
+KH_NORM_ROPE(bf16_v8_full, __nv_bfloat16, 8, 1, true)
+KH_NORM_ROPE(bf16_v8, __nv_bfloat16, 8, 1, false)
+KH_NORM_ROPE(bf16_v4, __nv_bfloat16, 4, 1, false)
+KH_NORM_ROPE(bf16_v1, __nv_bfloat16, 1, 4, false)
+KH_NORM_ROPE(f16_v8_full, __half, 8, 1, true)
+KH_NORM_ROPE(f16_v8, __half, 8, 1, false)
+KH_NORM_ROPE(f16_v4, __half, 4, 1, false)
+KH_NORM_ROPE(f16_v1, __half, 1, 4, false)
 
-// dw[k][i] = the sum over the blocks of partials[block][k][i]: a warp per 32 columns and eighth of the
-// blocks, the eighths added in order.
+// dw[k][i] = the sum of partials[block][i] over the blocks of queries (k = 0) or keys: a warp per 32 columns and
+// eighth of the blocks, the eighths added in order.
 extern "C" __global__ void __launch_bounds__(256) qk_norm_weight_grad(const __grid_constant__ WeightGradParams P) {
   __shared__ float part[8][32];
   khd::grid_dependency_wait();
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+  const int k = blockIdx.y, col = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+  const float *from = P.partials + static_cast<int64_t>(k == 0 ? 0 : P.blocks[0]) * P.head_dim;
   float v = 0.f;
-  if (col < 2 * P.head_dim)
-    for (int b = w; b < P.blocks; b += 8) v += P.partials[static_cast<int64_t>(b) * 2 * P.head_dim + col];
+  if (col < P.head_dim)
+#pragma unroll 8
+    for (int b = w; b < P.blocks[k]; b += 8) v += from[static_cast<int64_t>(b) * P.head_dim + col];
   part[w][threadIdx.x & 31] = v;
   __syncthreads();
-  if (w != 0 || col >= 2 * P.head_dim) return;
+  float *out = k == 0 ? P.dq_weight : P.dk_weight;
+  if (w != 0 || col >= P.head_dim || out == nullptr) return;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum += part[i][threadIdx.x];
-  const int k = col / P.head_dim, at = col - k * P.head_dim;
-  float *out = k == 0 ? P.dq_weight : P.dk_weight;
-  if (out != nullptr) out[at] = sum;
+  out[col] = sum;
 }

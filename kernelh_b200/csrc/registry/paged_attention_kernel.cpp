@@ -14,6 +14,7 @@ namespace {
 constexpr int kRows = 16, kUnit = 64;                  // kernels/paged_attention.cu
 constexpr int kChunkRows = 256, kChunkKeys = 128;      // kernels/paged_attention_chunk.cu
 constexpr int kMinUnits = 2;          // units per worker below which more workers cost more than they bring
+constexpr int kWholeKeys = 512;       // see run_paged_attention
 constexpr long kMaxSms = 160;         // workspaces are sized for at most this many SMs
 
 int element_size(int32_t dtype) { return dtype == KH_F32 ? 4 : 2; }
@@ -37,7 +38,7 @@ struct PagedParams {
   uint32_t *status;
   int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, page_shift, table_width, num_pages;
   int32_t causal, window;
-  int32_t workers, min_units;
+  int32_t workers, min_units, whole;
   int32_t rows_above, rows_upto;
   float scale_log2;
 };
@@ -71,9 +72,11 @@ bool chunk_kernel_fits(const kh_paged_attention_args &a) {
 bool many_rows(const kh_paged_attention_args &a) { return static_cast<int64_t>(a.max_q_len) * (a.q_heads / a.k_heads) > kRows; }
 
 // Grows with `sms` and with every length: the workspace, counted for kMaxSms, covers any device's launch.
+int64_t item_count(const kh_paged_attention_args &a, int rows) { // at most
+  return (a.tokens * (a.q_heads / a.k_heads) / rows + a.batch) * a.k_heads;
+}
 int64_t worker_count(const kh_paged_attention_args &a, int rows, int unit, int per_sm, long sms) {
-  const int64_t group = a.q_heads / a.k_heads;
-  const int64_t items = (a.tokens * group / rows + a.batch) * a.k_heads; // at most
+  const int64_t items = item_count(a, rows);
   const int64_t units = (static_cast<int64_t>(std::max(a.max_kv_len, 1)) + unit - 1) / unit;
   const int64_t most = per_sm * std::min(sms, kMaxSms);
   return std::min<int64_t>(most, std::max<int64_t>(1, (items * units + kMinUnits - 1) / kMinUnits));
@@ -242,11 +245,20 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
     if (alone) return {};
     p.rows_above = 0, p.rows_upto = kRows;
   }
-  const unsigned n = workers(kRows, kUnit, s.per_sm);
+  // Short key ranges are not split: an item takes less than the second launch that would add its parts up. (Replayed
+  // from a graph, 32 heads over 8 of 128 in bf16: 8 sequences of 200 keys 10.4 us against 13.4, 64 of 400 keys 27.1
+  // against 34.7, one of 800 keys 16.6 against 12.4, 64 of 800 keys 45.6 against 51.8.)
+  unsigned n = workers(kRows, kUnit, s.per_sm);
+  if (a.max_kv_len <= kWholeKeys || (a.max_kv_len <= 2 * kWholeKeys && item_count(a, kRows) >= s.per_sm * sms)) {
+    p.whole = 1;
+    p.min_units = 1;
+    n = static_cast<unsigned>(std::min<int64_t>(item_count(a, kRows), s.per_sm * sms)); // writes nothing to the workspace
+    p.workers = static_cast<int32_t>(n);
+  }
   if (auto r = launch("paged_attention", "paged_attention_" + suffix, {n, 1, 1}, 32u * s.warps, s.smem, {}, 0); !r) return r;
-  if (n == 1) return {};
+  if (n == 1 || p.whole) return {};
   const unsigned y = static_cast<unsigned>(std::min<int64_t>(kRows, all_rows)); // a row per block
-  return launch("paged_attention", "paged_attention_combine_" + suffix, {n - 1, y, 1}, 128, 0, {}, 0);
+  return launch("paged_attention", "paged_attention_combine_" + suffix, {n - 1, y, 1}, 256, 0, {}, 0);
 }
 
 } // namespace kh

@@ -13,7 +13,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxHeadDim = 256;
 // Blocks of the backward pass per SM and in all: one row of weight-gradient sums each.
-constexpr int kBackwardBlocksPerSm = 2, kBackwardMaxBlocks = 2 * 160;
+constexpr int kBackwardBlocksPerSm = 2, kBackwardMaxBlocks = 2 * 160, kForwardBlocksPerSm = 3;
+constexpr int kMaxAngles = 1024; // pairs x tokens of a tile (kernels/qk_norm_rope.cu)
 
 int element_size(int32_t dtype) { return dtype == KH_F32 ? 4 : 2; }
 
@@ -24,9 +25,11 @@ struct NormRopeParams {
   const int64_t *positions;
   int64_t tokens;
   int32_t q_heads, k_heads, head_dim, rotary_dim;
-  int32_t interleaved, lanes, tile_tokens;
+  int32_t lanes;
   float eps;
+  int32_t blocks[3], tile[3];
 };
+static_assert(sizeof(NormRopeParams) <= LaunchArgs::kMaxStructBytes);
 struct AppendParams {
   kh_head_rows v;
   kh_paged_rows k_cache, v_cache;
@@ -42,7 +45,7 @@ struct BackwardParams {
 struct WeightGradParams {
   const float *partials;
   float *dq_weight, *dk_weight;
-  int32_t blocks, head_dim;
+  int32_t blocks[2], head_dim;
 };
 
 // The stride of a dimension of size 1 says nothing.
@@ -104,7 +107,7 @@ int vector_width(const NormRopeCall &c) {
 } // namespace
 
 int64_t qk_norm_rope_backward_workspace(int32_t head_dim) {
-  return static_cast<int64_t>(kBackwardMaxBlocks) * 2 * std::max(head_dim, 0) * 4;
+  return static_cast<int64_t>(kBackwardMaxBlocks) * std::max(head_dim, 0) * 4;
 }
 
 Result<void> check_qk_norm_rope(const char *entry, const NormRopeCall &c) {
@@ -173,27 +176,35 @@ Result<void> run_qk_norm_rope(Executor &ex, NormRopeCall c, StreamHandle stream)
   }
   long sms = query_cu_count(ex.limits());
   if (sms <= 0) sms = 148;
-  int blocks = 0;
+  NormRopeParams p{};
   if (a.tokens > 0) {
     const int vec = vector_width(c), slots = vec == 1 ? 4 : 1;
     const int pair_vectors = (a.head_dim / 2 + vec - 1) / vec;
-    NormRopeParams p{};
     p.q = a.q, p.k = a.k, p.q_out = c.q_out, p.k_out = c.k_out;
     p.q_weight = a.q_weight, p.k_weight = a.k_weight, p.inv_freq = a.inv_freq, p.positions = a.positions;
     p.tokens = a.tokens;
     p.q_heads = a.q_heads, p.k_heads = a.k_heads, p.head_dim = a.head_dim, p.rotary_dim = a.rotary_dim;
-    p.interleaved = a.interleaved;
     p.eps = a.eps;
     p.lanes = static_cast<int>(std::bit_ceil(static_cast<unsigned>((pair_vectors + slots - 1) / slots)));
-    // Four tokens share a block (and its 256 angles) once that still leaves two blocks per SM.
-    p.tile_tokens = a.tokens >= 4 * 2 * sms ? 4 : 1;
-    const int64_t tiles = (a.tokens + p.tile_tokens - 1) / p.tile_tokens;
+    // Blocks go to queries, keys and values by their share of the rows, at least one each and none without a tile. A
+    // tile has about four rows for every group of lanes, fewer where that would leave blocks without one.
+    const int kinds = append ? 3 : 2, groups = kThreads / p.lanes;
+    const int64_t most = backward ? std::min<int64_t>(kBackwardBlocksPerSm * sms, kBackwardMaxBlocks) : kForwardBlocksPerSm * sms;
+    const int64_t heads[3] = {a.q_heads, a.k_heads, a.k_heads}, all = a.q_heads + (kinds - 1) * static_cast<int64_t>(a.k_heads);
+    int64_t blocks = 0;
+    for (int i = 0; i < kinds; ++i) {
+      const int64_t share = std::max<int64_t>(1, most * heads[i] / all);
+      p.tile[i] = static_cast<int32_t>(std::max<int64_t>(1, std::min({4 * groups / heads[i], static_cast<int64_t>(kMaxAngles / (a.head_dim / 2)), a.tokens / share})));
+      p.blocks[i] = static_cast<int32_t>(std::min(share, (a.tokens + p.tile[i] - 1) / p.tile[i]));
+      blocks += p.blocks[i];
+    }
     LaunchStep step;
     step.entry = std::string(append ? "qk_norm_rope_append_" : backward ? "qk_norm_rope_backward_" : "qk_norm_rope_") +
-                 (a.dtype == KH_F32 ? "f32_v" : a.dtype == KH_BF16 ? "bf16_v" : "f16_v") + std::to_string(vec);
+                 (a.dtype == KH_F32 ? "f32_v" : a.dtype == KH_BF16 ? "bf16_v" : "f16_v") + std::to_string(vec) +
+                 (vec * element_size(a.dtype) == 16 && pair_vectors == p.lanes ? "_full" : "") + (a.interleaved ? "_inter" : "_halves");
     step.block = {kThreads, 1, 1};
     step.overlap_tail = true;
-    step.grid = {static_cast<unsigned>(tiles), 1, 1};
+    step.grid = {static_cast<unsigned>(blocks), 1, 1};
     LaunchArgs args;
     args.add_struct_bytes(&p, sizeof p);
     if (append) {
@@ -201,8 +212,6 @@ Result<void> run_qk_norm_rope(Executor &ex, NormRopeCall c, StreamHandle stream)
       args.add_struct_bytes(&q, sizeof q);
     }
     if (backward) {
-      blocks = static_cast<int>(std::min<int64_t>({tiles, kBackwardBlocksPerSm * sms, kBackwardMaxBlocks}));
-      step.grid = {static_cast<unsigned>(blocks), 1, 1};
       const BackwardParams q{c.dq_out, c.dk_out, static_cast<float *>(c.workspace)};
       args.add_struct_bytes(&q, sizeof q);
     }
@@ -215,12 +224,12 @@ Result<void> run_qk_norm_rope(Executor &ex, NormRopeCall c, StreamHandle stream)
   LaunchStep step;
   step.entry = "qk_norm_weight_grad";
   step.block = {256, 1, 1};
-  step.grid = {static_cast<unsigned>((2 * a.head_dim + 31) / 32), 1, 1};
+  step.grid = {static_cast<unsigned>((a.head_dim + 31) / 32), 2, 1};
   step.overlap_tail = true;
   step.param_count = 1;
-  const WeightGradParams p{static_cast<const float *>(c.workspace), c.dq_weight, c.dk_weight, blocks, a.head_dim};
+  const WeightGradParams q{static_cast<const float *>(c.workspace), c.dq_weight, c.dk_weight, {p.blocks[0], p.blocks[1]}, a.head_dim};
   LaunchArgs args;
-  args.add_struct_bytes(&p, sizeof p);
+  args.add_struct_bytes(&q, sizeof q);
   auto fn = ex.function("qk_norm_rope", step.entry);
   if (!fn) return std::unexpected(fn.error());
   return ex.launch(*fn, step, args, stream);
