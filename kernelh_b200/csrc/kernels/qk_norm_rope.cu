@@ -15,14 +15,16 @@
 // row is read and written by the same lanes, read first: outputs may be the inputs themselves.
 //
 // A persistent grid whose blocks are dealt out to queries, keys (and values) by their share of the rows, so
-// that a block has one weight, kept in registers, and one set of weight-gradient sums. A block takes tiles of
+// that a block has one weight and one set of weight-gradient sums. A block takes tiles of
 // tokens; its groups walk the tile's rows, the next row's loads in flight while one is worked on.
 // Angles: position * inv_freq in half turns, formed and reduced in 64 bits (a position of 10^6 times a
 // frequency of 1 has 20 bits before the point, fp32 would keep 4 after it), the remainder in [-1, 1]
 // rounded to fp32 for sincospif. They are worked out once per tile by the whole block into shared memory and
 // shared by all its heads: 50 instructions each, which every row on its own would pay again. Arithmetic on
 // pairs of values (fp32x2) and packed conversions: the kernels are bound by instructions before they are bound
-// by HBM (32768 tokens x 40 heads x 128 bf16: 370 instructions per row and warp, 202 us, before; MEASURE now).
+// by HBM. Measured: 32768 tokens x 40 heads x 128 bf16 in 127 us, 5.3 TB/s (202 us with scalar arithmetic and every
+// group computing addresses for three tensors, 370 instructions for four rows of a warp); 16384 x 40 x 128 fp32 in 112 us,
+// 6.0 TB/s; backward of 16384 x 40 x 128 in 105 us (bf16, 4.8 TB/s) and 165 us (fp32, 6.1 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -32,6 +34,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxAngles = 1024; // pairs x tokens of a tile
+// Blocks per SM (the host's grid counts on them). A lane of a 16-bit row holds twice the values: one block more spills
+// (bf16 forward 127 -> 139 us, backward 105 -> 141 at the sizes above; fp32 118 -> 111 and 183 -> 165).
+template <typename T> constexpr int kForwardBlocks = sizeof(T) == 4 ? 4 : 3;
+template <typename T> constexpr int kBackwardBlocks = sizeof(T) == 4 ? 3 : 2;
 
 // Rows of head_dim contiguous values: data + token * token_stride + head * head_stride (elements).
 struct HeadRows {
@@ -150,7 +156,7 @@ template <typename T_, int kVec_, int kSlots_, bool kFull_, bool kInterleaved_> 
       }
   }
   // Zeros for slots that are off.
-  __device__ __forceinline__ void widen(const RawT &v, bool mine, Values &x) const {
+  __device__ __forceinline__ void widen(const RawT &v, Values &x) const {
     float a[kPairs], b[kPairs];
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
@@ -170,7 +176,7 @@ template <typename T_, int kVec_, int kSlots_, bool kFull_, bool kInterleaved_> 
           y[2 * i] = p.x, y[2 * i + 1] = p.y, y[kVec + 2 * i] = q.x, y[kVec + 2 * i + 1] = q.y;
         }
       }
-      const bool keep = kFull ? mine : mine && on[s];
+      const bool keep = kFull || on[s];
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
         a[s * kVec + i] = keep ? y[kInterleaved ? 2 * i : i] : 0.f;
@@ -213,27 +219,11 @@ template <typename T_, int kVec_, int kSlots_, bool kFull_, bool kInterleaved_> 
       }
     }
   }
-  // Values of a head_dim vector (a weight; a null one is all ones) that belong to this lane's pairs.
-  __device__ __forceinline__ void weights(const float *w, Values &x) const {
-    float a[kPairs], b[kPairs];
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s)
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        a[s * kVec + i] = w != nullptr && on[s] ? __ldg(w + at(s, i, false)) : 1.f;
-        b[s * kVec + i] = w != nullptr && on[s] ? __ldg(w + at(s, i, true)) : 1.f;
-      }
-#pragma unroll
-    for (int i = 0; i < kPairs / 2; ++i) {
-      x.a[i] = make_float2(a[2 * i], a[2 * i + 1]);
-      x.b[i] = make_float2(b[2 * i], b[2 * i + 1]);
-    }
-  }
   __device__ __forceinline__ int at(int s, int i, bool second) const {
     return kInterleaved ? at_a[s] + 2 * i + second : (second ? at_b[s] : at_a[s]) + i;
   }
-  // cos and sin of this lane's pairs out of a token's table.
-  __device__ __forceinline__ void angles(const float *cs, const float *sn, float2 (&c)[kPairs / 2], float2 (&s)[kPairs / 2]) const {
+  // This lane's values out of two tables by pair (cos and sin of a token; the weights of both values).
+  __device__ __forceinline__ void look_up(const float *cs, const float *sn, float2 (&c)[kPairs / 2], float2 (&s)[kPairs / 2]) const {
     float fc[kPairs], fs[kPairs];
 #pragma unroll
     for (int x = 0; x < kSlots; ++x) {
@@ -259,28 +249,28 @@ template <typename T_, int kVec_, int kSlots_, bool kFull_, bool kInterleaved_> 
   }
   // Turns the pairs by their angles (`sign` -1: back). Pairs from `half` on stay exactly as they are.
   template <int sign> __device__ __forceinline__ void rotate(Values &x, const float2 (&c)[kPairs / 2], const float2 (&s)[kPairs / 2], int half) const {
-    bool all = true;
-#pragma unroll
-    for (int y = 0; y < kSlots; ++y) all = all && first[y] + kVec <= half;
+    if (kSlots == 1 && first[0] >= half) return;
+    const bool all = kSlots == 1 && first[0] + kVec <= half;
+    const Values old = x;
 #pragma unroll
     for (int i = 0; i < kPairs / 2; ++i) {
       const float2 p = x.a[i], q = x.b[i];
       const float2 qs = __fmul2_rn(q, s[i]), ps = __fmul2_rn(p, s[i]);
-      float2 a, b;
       if (sign > 0) {
-        a = make_float2(fmaf(p.x, c[i].x, -qs.x), fmaf(p.y, c[i].y, -qs.y));
-        b = __ffma2_rn(q, c[i], ps);
+        x.a[i] = make_float2(fmaf(p.x, c[i].x, -qs.x), fmaf(p.y, c[i].y, -qs.y));
+        x.b[i] = __ffma2_rn(q, c[i], ps);
       } else {
-        a = __ffma2_rn(p, c[i], qs);
-        b = make_float2(fmaf(q.x, c[i].x, -ps.x), fmaf(q.y, c[i].y, -ps.y));
+        x.a[i] = __ffma2_rn(p, c[i], qs);
+        x.b[i] = make_float2(fmaf(q.x, c[i].x, -ps.x), fmaf(q.y, c[i].y, -ps.y));
       }
-      if (!all) {
+    }
+    if (!all) { // a lane that holds pairs of both kinds
+#pragma unroll
+      for (int i = 0; i < kPairs / 2; ++i) {
         const bool x0 = first[2 * i / kVec] + 2 * i % kVec < half, x1 = first[(2 * i + 1) / kVec] + (2 * i + 1) % kVec < half;
-        a = make_float2(x0 ? a.x : p.x, x1 ? a.y : p.y);
-        b = make_float2(x0 ? b.x : q.x, x1 ? b.y : q.y);
+        x.a[i] = make_float2(x0 ? x.a[i].x : old.a[i].x, x1 ? x.a[i].y : old.a[i].y);
+        x.b[i] = make_float2(x0 ? x.b[i].x : old.b[i].x, x1 ? x.b[i].y : old.b[i].y);
       }
-      x.a[i] = a;
-      x.b[i] = b;
     }
   }
 };
@@ -303,6 +293,9 @@ template <int kPairs> __device__ __forceinline__ float dot(const Pairs<kPairs> &
 }
 
 // cos and sin of every pair of the tile's tokens, (1, 0) past the rotated part.
+// For 16-bit rows sin and cos come from the special-function units (error below 2^-21 of 1 in [-pi, pi], where the
+// outputs keep 2^-12 at best); with few heads the angles are most of the work (32768 tokens x 9 heads 98 -> 51 us).
+template <typename T>
 __device__ __forceinline__ void fill_angles(const NormRopeParams &P, int64_t token0, int tokens, float *cs, float *sn) {
   const int pairs = P.head_dim >> 1, half = P.rotary_dim >> 1;
   for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
@@ -310,10 +303,23 @@ __device__ __forceinline__ void fill_angles(const NormRopeParams &P, int64_t tok
     float c = 1.f, s = 0.f;
     if (j < half) {
       const double turns = static_cast<double>(P.positions[token0 + t]) * static_cast<double>(P.inv_freq[j]) * 0.31830988618379067154;
-      sincospif(static_cast<float>(turns - 2.0 * rint(0.5 * turns)), &s, &c);
+      const float rest = static_cast<float>(turns - 2.0 * rint(0.5 * turns));
+      if (sizeof(T) == 4) sincospif(rest, &s, &c);
+      else __sincosf(rest * 3.14159265358979f, &s, &c);
     }
     cs[i] = c;
     sn[i] = s;
+  }
+}
+
+// The block's weight into shared memory, by pair; a null one is all ones. The barrier is the caller's first.
+template <bool kInterleaved> __device__ __forceinline__ void fetch_weight(const float *w, const NormRopeParams &P, float (*to)[128]) {
+  const int half = P.rotary_dim >> 1;
+  for (int j = threadIdx.x; j < P.head_dim >> 1; j += kThreads) {
+    const int a = kInterleaved ? 2 * j : j < half ? j : P.rotary_dim + j - half;
+    const int b = kInterleaved ? 2 * j + 1 : a + (j < half ? half : (P.head_dim - P.rotary_dim) >> 1);
+    to[0][j] = w != nullptr ? w[a] : 1.f;
+    to[1][j] = w != nullptr ? w[b] : 1.f;
   }
 }
 
@@ -338,22 +344,29 @@ struct Share {
     token_first = group / heads;
     head_first = group % heads;
   }
-  __device__ __forceinline__ void next(int &token, int &head) const {
-    token += token_step;
-    head += head_step;
-    if (head >= heads) {
-      head -= heads;
+};
+// A group's walk through the rows of a tile.
+struct Place {
+  int token, head;
+  __device__ __forceinline__ Place(const Share &me) : token(me.token_first), head(me.head_first) {}
+  __device__ __forceinline__ void next(const Share &me) {
+    token += me.token_step;
+    head += me.head_step;
+    if (head >= me.heads) {
+      head -= me.heads;
       ++token;
     }
   }
+  template <typename T> __device__ __forceinline__ T *in(T *base, const HeadRows &rows) const { return base + token * rows.token_stride + head * rows.head_stride; }
 };
-template <typename T> __device__ __forceinline__ T *row_of(const HeadRows &rows, int64_t token, int head) {
-  return reinterpret_cast<T *>(rows.data) + token * rows.token_stride + head * rows.head_stride;
+template <typename T> __device__ __forceinline__ T *tile_of(const HeadRows &rows, int64_t token0) {
+  return reinterpret_cast<T *>(rows.data) + token0 * rows.token_stride;
 }
 
 template <typename L, bool kAppend> __device__ __forceinline__ void forward_body(const NormRopeParams &P, const AppendParams &A) {
   using T = typename L::T;
   __shared__ __align__(16) float s_cos[2][kMaxAngles], s_sin[2][kMaxAngles];
+  __shared__ __align__(16) float s_weight[2][128];
   __shared__ int64_t s_place[2][kAppend ? kMaxAngles : 1]; // where the token's rows go in the cache (INT64_MIN: nowhere)
   const Share me(P);
   const L lay(P, me.lane);
@@ -364,16 +377,20 @@ template <typename L, bool kAppend> __device__ __forceinline__ void forward_body
   const HeadRows in = me.kind == 0 ? P.q : me.kind == 1 ? P.k : A.v;
   const HeadRows out = me.kind == 0 ? P.q_out : P.k_out;
   const PagedRows cache = me.kind == 1 ? A.k_cache : A.v_cache;
-  typename L::Values w;
-  lay.weights(me.kind == 0 ? P.q_weight : me.kind == 1 ? P.k_weight : nullptr, w);
+  fetch_weight<L::kInterleaved>(me.kind == 0 ? P.q_weight : P.k_weight, P, s_weight);
   const int64_t tiles = (P.tokens + me.tile - 1) / me.tile;
   int buffer = 0;
   for (int64_t tile = me.block; tile < tiles; tile += me.blocks, buffer ^= 1) {
     const int64_t token0 = tile * me.tile;
     const int tokens = static_cast<int>(min(static_cast<int64_t>(me.tile), P.tokens - token0)), rows = tokens * me.heads;
-    typename L::RawT raw;
-    int t = me.token_first, h = me.head_first;
-    if (me.group < rows) lay.load(row_of<T>(in, token0 + t, h), raw);
+    typename L::RawT raw[2]; // the next row and the one after it
+    T *const in_tile = tile_of<T>(in, token0), *const out_tile = tile_of<T>(out, token0);
+    Place at(me), ahead(me);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (me.group + i * me.groups < rows) lay.load(ahead.in(in_tile, in), raw[i]);
+      ahead.next(me);
+    }
     if (kAppend && me.kind > 0) {
       for (int i = threadIdx.x; i < tokens; i += kThreads) {
         const int64_t slot = A.slots[token0 + i];
@@ -387,22 +404,24 @@ template <typename L, bool kAppend> __device__ __forceinline__ void forward_body
         s_place[buffer][i] = place;
       }
     }
-    if (me.kind < 2) fill_angles(P, token0, tokens, s_cos[buffer], s_sin[buffer]);
+    if (me.kind < 2) fill_angles<T>(P, token0, tokens, s_cos[buffer], s_sin[buffer]);
     __syncthreads(); // the other buffers' readers passed the barrier before this one
     // every lane of a warp makes the same number of turns, so that the shuffles are always complete
     for (int r0 = 0; r0 < rows; r0 += me.groups) {
       const bool mine = r0 + me.group < rows;
-      typename L::RawT cur = raw;
-      int t_next = t, h_next = h;
-      me.next(t_next, h_next);
-      if (r0 + me.groups + me.group < rows) lay.load(row_of<T>(in, token0 + t_next, h_next), raw);
+      typename L::RawT cur = raw[0];
+      raw[0] = raw[1];
+      if (r0 + 2 * me.groups + me.group < rows) lay.load(ahead.in(in_tile, in), raw[1]);
+      ahead.next(me);
       if (!kAppend || me.kind < 2) {
         typename L::Values x;
-        lay.widen(cur, mine, x);
+        lay.widen(cur, x); // (a group without a row works on what its registers hold, among its own lanes)
         const float r = rsqrtf(fmaf(group_sum(dot(x, x), P.lanes), scale, P.eps));
         if (mine) {
           float2 c[L::kPairs / 2], s[L::kPairs / 2];
-          lay.angles(s_cos[buffer] + t * pairs, s_sin[buffer] + t * pairs, c, s);
+          lay.look_up(s_cos[buffer] + at.token * pairs, s_sin[buffer] + at.token * pairs, c, s);
+          typename L::Values w;
+          lay.look_up(s_weight[0], s_weight[1], w.a, w.b);
           const float2 r2 = make_float2(r, r);
 #pragma unroll
           for (int i = 0; i < L::kPairs / 2; ++i) {
@@ -415,13 +434,12 @@ template <typename L, bool kAppend> __device__ __forceinline__ void forward_body
       }
       if (mine) {
         if (!kAppend || me.kind == 0) {
-          lay.store(row_of<T>(out, token0 + t, h), cur);
-        } else if (const int64_t place = s_place[buffer][t]; place != INT64_MIN) {
-          lay.store(reinterpret_cast<T *>(cache.data) + place + h * cache.head_stride, cur);
+          lay.store(at.in(out_tile, out), cur);
+        } else if (const int64_t place = s_place[buffer][at.token]; place != INT64_MIN) {
+          lay.store(reinterpret_cast<T *>(cache.data) + place + at.head * cache.head_stride, cur);
         }
       }
-      t = t_next;
-      h = h_next;
+      at.next(me);
     }
   }
 }
@@ -432,6 +450,7 @@ template <typename L, bool kAppend> __device__ __forceinline__ void forward_body
 template <typename L> __device__ __forceinline__ void backward_body(const NormRopeParams &P, const BackwardParams &B) {
   using T = typename L::T;
   __shared__ __align__(16) float s_cos[2][kMaxAngles], s_sin[2][kMaxAngles];
+  __shared__ __align__(16) float s_weight[2][128];
   __shared__ float s_sum[kThreads / 32][256];
   const Share me(P);
   const L lay(P, me.lane);
@@ -440,8 +459,8 @@ template <typename L> __device__ __forceinline__ void backward_body(const NormRo
   khd::grid_dependency_wait();
   khd::grid_dependents_may_launch();
   const HeadRows in = me.kind == 0 ? P.q : P.k, grad = me.kind == 0 ? B.dq_out : B.dk_out, out = me.kind == 0 ? P.q_out : P.k_out;
-  typename L::Values w, sum;
-  lay.weights(me.kind == 0 ? P.q_weight : P.k_weight, w);
+  fetch_weight<L::kInterleaved>(me.kind == 0 ? P.q_weight : P.k_weight, P, s_weight);
+  typename L::Values sum;
 #pragma unroll
   for (int i = 0; i < L::kPairs / 2; ++i) sum.a[i] = sum.b[i] = make_float2(0.f, 0.f);
   const int64_t tiles = (P.tokens + me.tile - 1) / me.tile;
@@ -450,36 +469,40 @@ template <typename L> __device__ __forceinline__ void backward_body(const NormRo
     const int64_t token0 = tile * me.tile;
     const int tokens = static_cast<int>(min(static_cast<int64_t>(me.tile), P.tokens - token0)), rows = tokens * me.heads;
     typename L::RawT raw, draw;
-    int t = me.token_first, h = me.head_first;
+    T *const in_tile = tile_of<T>(in, token0), *const grad_tile = tile_of<T>(grad, token0), *const out_tile = tile_of<T>(out, token0);
+    Place at(me), ahead(me);
     if (me.group < rows) {
-      lay.load(row_of<T>(in, token0 + t, h), raw);
-      lay.load(row_of<T>(grad, token0 + t, h), draw);
+      lay.load(ahead.in(in_tile, in), raw);
+      lay.load(ahead.in(grad_tile, grad), draw);
     }
-    fill_angles(P, token0, tokens, s_cos[buffer], s_sin[buffer]);
+    fill_angles<T>(P, token0, tokens, s_cos[buffer], s_sin[buffer]);
     __syncthreads(); // the other buffer's readers passed the barrier before this one
     for (int r0 = 0; r0 < rows; r0 += me.groups) {
       const bool mine = r0 + me.group < rows;
       typename L::Values u, g;
-      lay.widen(raw, mine, u);
-      lay.widen(draw, mine, g);
-      int t_next = t, h_next = h;
-      me.next(t_next, h_next);
+      lay.widen(raw, u); // (a group without a row works on what its registers hold, among its own lanes)
+      lay.widen(draw, g);
+      ahead.next(me);
       if (r0 + me.groups + me.group < rows) {
-        lay.load(row_of<T>(in, token0 + t_next, h_next), raw);
-        lay.load(row_of<T>(grad, token0 + t_next, h_next), draw);
+        lay.load(ahead.in(in_tile, in), raw);
+        lay.load(ahead.in(grad_tile, grad), draw);
       }
       const float r = rsqrtf(fmaf(group_sum(dot(u, u), P.lanes), scale, P.eps));
       const float2 r2 = make_float2(r, r);
       float2 c[L::kPairs / 2], s[L::kPairs / 2];
-      const int at = (mine ? t : 0) * pairs;
-      lay.angles(s_cos[buffer] + at, s_sin[buffer] + at, c, s);
+      const int table = (mine ? at.token : 0) * pairs;
+      lay.look_up(s_cos[buffer] + table, s_sin[buffer] + table, c, s);
       lay.template rotate<-1>(g, c, s, half);
+      typename L::Values w;
+      lay.look_up(s_weight[0], s_weight[1], w.a, w.b);
 #pragma unroll
       for (int i = 0; i < L::kPairs / 2; ++i) {
         u.a[i] = __fmul2_rn(u.a[i], r2);
         u.b[i] = __fmul2_rn(u.b[i], r2);
-        sum.a[i] = __ffma2_rn(g.a[i], u.a[i], sum.a[i]);
-        sum.b[i] = __ffma2_rn(g.b[i], u.b[i], sum.b[i]);
+        if (mine) {
+          sum.a[i] = __ffma2_rn(g.a[i], u.a[i], sum.a[i]);
+          sum.b[i] = __ffma2_rn(g.b[i], u.b[i], sum.b[i]);
+        }
         g.a[i] = __fmul2_rn(g.a[i], w.a[i]);
         g.b[i] = __fmul2_rn(g.b[i], w.b[i]);
       }
@@ -493,10 +516,9 @@ template <typename L> __device__ __forceinline__ void backward_body(const NormRo
         }
         typename L::RawT res;
         lay.narrow(g, res);
-        lay.store(row_of<T>(out, token0 + t, h), res);
+        lay.store(at.in(out_tile, out), res);
       }
-      t = t_next;
-      h = h_next;
+      at.next(me);
     }
   }
   // groups of a warp first (shuffles over the lanes that hold the same values), then the eight warps
@@ -524,15 +546,15 @@ template <typename L> __device__ __forceinline__ void backward_body(const NormRo
 } // namespace
 
 #define KH_NORM_ROPE_PAIRING(suffix, T, vec, slots, full, pairing)                                                      \
-  extern "C" __global__ void __launch_bounds__(kThreads, 3)                                                             \
+  extern "C" __global__ void __launch_bounds__(kThreads, kForwardBlocks<T>)                                                             \
   qk_norm_rope_##suffix(const __grid_constant__ NormRopeParams P) {                                                     \
     forward_body<Layout<T, vec, slots, full, pairing>, false>(P, AppendParams{});                                       \
   }                                                                                                                     \
-  extern "C" __global__ void __launch_bounds__(kThreads, 3)                                                             \
+  extern "C" __global__ void __launch_bounds__(kThreads, kForwardBlocks<T>)                                                             \
   qk_norm_rope_append_##suffix(const __grid_constant__ NormRopeParams P, const __grid_constant__ AppendParams A) {      \
     forward_body<Layout<T, vec, slots, full, pairing>, true>(P, A);                                                     \
   }                                                                                                                     \
-  extern "C" __global__ void __launch_bounds__(kThreads, 2)                                                             \
+  extern "C" __global__ void __launch_bounds__(kThreads, kBackwardBlocks<T>)                                                             \
   qk_norm_rope_backward_##suffix(const __grid_constant__ NormRopeParams P, const __grid_constant__ BackwardParams B) {  \
     backward_body<Layout<T, vec, slots, full, pairing>>(P, B);                                                          \
   }

@@ -12,8 +12,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHeadDim = 256;
-// Blocks of the backward pass per SM and in all: one row of weight-gradient sums each.
-constexpr int kBackwardBlocksPerSm = 2, kBackwardMaxBlocks = 2 * 160, kForwardBlocksPerSm = 3;
+// Blocks per SM (as the kernels are bounded: a wide row's lane holds half the values), and at most in the backward
+// pass, where each leaves a row of weight-gradient sums.
+constexpr int forward_blocks(int32_t dtype) { return dtype == KH_F32 ? 4 : 3; }
+constexpr int backward_blocks(int32_t dtype) { return dtype == KH_F32 ? 3 : 2; }
+constexpr int kBackwardMaxBlocks = 3 * 160;
 constexpr int kMaxAngles = 1024; // pairs x tokens of a tile (kernels/qk_norm_rope.cu)
 
 int element_size(int32_t dtype) { return dtype == KH_F32 ? 4 : 2; }
@@ -186,16 +189,19 @@ Result<void> run_qk_norm_rope(Executor &ex, NormRopeCall c, StreamHandle stream)
     p.q_heads = a.q_heads, p.k_heads = a.k_heads, p.head_dim = a.head_dim, p.rotary_dim = a.rotary_dim;
     p.eps = a.eps;
     p.lanes = static_cast<int>(std::bit_ceil(static_cast<unsigned>((pair_vectors + slots - 1) / slots)));
-    // Blocks go to queries, keys and values by their share of the rows, at least one each and none without a tile. A
-    // tile has about four rows for every group of lanes, fewer where that would leave blocks without one.
+    // Blocks go to queries, keys and values by their rows, a token's angles counting as four of them: at least one
+    // each and none without a tile. A tile has at most about eight rows for every group of lanes, and every block the
+    // same number of tiles or one less.
     const int kinds = append ? 3 : 2, groups = kThreads / p.lanes;
-    const int64_t most = backward ? std::min<int64_t>(kBackwardBlocksPerSm * sms, kBackwardMaxBlocks) : kForwardBlocksPerSm * sms;
-    const int64_t heads[3] = {a.q_heads, a.k_heads, a.k_heads}, all = a.q_heads + (kinds - 1) * static_cast<int64_t>(a.k_heads);
+    const int64_t most = backward ? std::min<int64_t>(backward_blocks(a.dtype) * sms, kBackwardMaxBlocks) : forward_blocks(a.dtype) * sms;
+    const int64_t heads[3] = {a.q_heads, a.k_heads, a.k_heads}, cost[3] = {a.q_heads + 4, a.k_heads + 4, append ? a.k_heads : 0};
+    const auto pieces = [](int64_t n, int64_t size) { return (n + size - 1) / size; };
     int64_t blocks = 0;
     for (int i = 0; i < kinds; ++i) {
-      const int64_t share = std::max<int64_t>(1, most * heads[i] / all);
-      p.tile[i] = static_cast<int32_t>(std::max<int64_t>(1, std::min({4 * groups / heads[i], static_cast<int64_t>(kMaxAngles / (a.head_dim / 2)), a.tokens / share})));
-      p.blocks[i] = static_cast<int32_t>(std::min(share, (a.tokens + p.tile[i] - 1) / p.tile[i]));
+      const int64_t share = std::max<int64_t>(1, most * cost[i] / (cost[0] + cost[1] + cost[2]));
+      const int64_t largest = std::max<int64_t>(1, std::min<int64_t>(8 * groups / heads[i], kMaxAngles / (a.head_dim / 2)));
+      p.tile[i] = static_cast<int32_t>(pieces(a.tokens, share * pieces(a.tokens, share * largest)));
+      p.blocks[i] = static_cast<int32_t>(std::min(share, pieces(a.tokens, p.tile[i])));
       blocks += p.blocks[i];
     }
     LaunchStep step;
