@@ -205,6 +205,7 @@ def _ptr(x) -> int | None:
 # dtype codes of the entry points that take rows of more than one type, by the name torch gives the type
 _DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
 _dtype_codes: dict = {}  # the same by dtype object, filled as types are met (str() of a dtype is slow)
+_dtype_names: dict = {}  # their names, likewise
 
 
 def _refuse(message: str):
@@ -219,6 +220,13 @@ def _dtype_code(t, name: str) -> int:
             _refuse(f"'{name}' must be float32, bfloat16 or float16, got {t.dtype}")
         _dtype_codes[t.dtype] = code
     return code
+
+
+def _dtype_name(t) -> str:
+    name = _dtype_names.get(t.dtype)
+    if name is None:
+        name = _dtype_names[t.dtype] = str(t.dtype)
+    return name
 
 
 def shape_text(**shape: int) -> str:
@@ -404,7 +412,7 @@ class Context:
         """Address of a contiguous vector on this context's device, of `dtype` and `size` values."""
         if t.get_device() != self._ordinal:  # -1 for a tensor in host memory
             _refuse(f"'{name}' must be on device {self._ordinal} of this context, got {t.device}")
-        if dtype is not None and str(t.dtype) != dtype:
+        if dtype is not None and _dtype_name(t) != dtype:
             _refuse(f"'{name}' must be {dtype}, got {t.dtype}")
         if size is not None and t.numel() != size:
             _refuse(f"'{name}' must have {size} values, got {t.numel()}")
@@ -414,11 +422,11 @@ class Context:
 
     def _rows(self, t, name: str, shape, code: int) -> HeadRows:
         """A [tokens, heads, head_dim] tensor as rows: any strides but the last, which must be 1."""
-        if t.get_device() != self._ordinal:  # -1 for a tensor in host memory
+        if t.get_device() != self._ordinal:
             _refuse(f"'{name}' must be on device {self._ordinal} of this context, got {t.device}")
         if t.shape != shape:
             _refuse(f"'{name}' must have shape {tuple(shape)}, got {tuple(t.shape)}")
-        if _dtype_code(t, name) != code:
+        if _dtype_codes.get(t.dtype) != code:
             _refuse(f"'{name}' must have the type of 'q', got {t.dtype}")
         s0, s1, s2 = t.stride()
         if s2 != 1 and shape[2] != 1:
@@ -427,11 +435,11 @@ class Context:
 
     def _cache(self, t, name: str, shape, code: int) -> PagedRows:
         """A [pages, page_size, heads, head_dim] tensor as a paged cache: any strides but the last."""
-        if t.get_device() != self._ordinal:  # -1 for a tensor in host memory
+        if t.get_device() != self._ordinal:
             _refuse(f"'{name}' must be on device {self._ordinal} of this context, got {t.device}")
-        if t.dim() != 4 or tuple(t.shape) != shape:
-            _refuse(f"'{name}' must have shape {shape}, got {tuple(t.shape)}")
-        if _dtype_code(t, name) != code:
+        if t.shape != shape:
+            _refuse(f"'{name}' must have shape {tuple(shape)}, got {tuple(t.shape)}")
+        if _dtype_codes.get(t.dtype) != code:
             _refuse(f"'{name}' must have the type of 'q', got {t.dtype}")
         s0, s1, s2, s3 = t.stride()
         if s3 != 1 and shape[3] != 1:
@@ -519,7 +527,7 @@ class Context:
         code = _dtype_code(q, "q")
         tokens, q_heads, head_dim = q.shape
         pages, page_size, k_heads, _ = k_cache.shape
-        if page_table.dim() != 2 or str(page_table.dtype) != "torch.int32" or page_table.stride(1) != 1:
+        if page_table.dim() != 2 or _dtype_name(page_table) != "torch.int32" or page_table.stride(1) != 1:
             _refuse("'page_table' must be int32 [batch, width] with contiguous rows")
         if page_table.get_device() != self._ordinal:
             _refuse(f"'page_table' must be on device {self._ordinal} of this context, got {page_table.device}")

@@ -6,15 +6,16 @@
 // kRows of them; a query head never needs a tile of its own, so a single token with 8 query heads per
 // key/value head reads its keys and values once.
 //
-// Work. An item is (sequence, key/value head, row block) and takes n units of kUnit keys, n the same for all
-// items of a sequence (its whole key range; the causal mask cuts the units at an item's end, which cost
-// nothing), and kPad more that stand for its start and end. All of these of all items form one line, and every
-// worker (a block) takes an equal stretch of it, whatever the lengths are: a worker finishes the item it starts in, does whole ones, and leaves the last one
-// to the next worker. Items that more than one worker touches leave (max, sum, unnormalised row) in the
-// workspace: slot 2w + 1 for the worker that starts an item, 2w for those that continue it. The first worker
-// that begins inside an item also leaves a note of it, and a second launch adds the parts up in the order of
-// the keys. The line is laid out from q_start and kv_len on the device, so a
-// captured call follows lengths that change between replays.
+// Work. An item is (sequence, key/value head, row block) and takes n units of kUnit keys: from the first key that
+// any of its rows sees to the last. With a few more that stand for its start and end, the units of all items form one
+// line, and every worker (a block) takes an equal stretch of it, whatever the lengths are: a worker finishes the item
+// it starts in, does whole ones, and leaves the last one to the next worker. Under the causal mask the blocks of a
+// sequence differ in length; they lie on the line in pairs, shortest with longest, whose sum is nearly the same for
+// all, so that a place on the line still leads to its item by one division. Items that more than one worker touches
+// leave (max, sum, unnormalised row) in the workspace: slot 2w + 1 for the worker that starts an item, 2w for those
+// that continue it. The first worker that begins inside an item also leaves a note of it, and a second launch adds the
+// parts up in the order of the keys. The line is laid out from q_start and kv_len on the device, so a captured call
+// follows lengths that change between replays.
 #pragma once
 
 #include "kh_device.cuh"
@@ -39,23 +40,48 @@ struct PagedParams {
   float2 *partial_ml;
   struct SplitItem *split_items; // [workers]
   uint32_t *status;
-  int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, page_shift, table_width, num_pages; // page_size = 2^page_shift, or page_shift < 0
+  int32_t tokens, batch, k_heads, group, head_dim, page_size, page_shift, table_width, num_pages; // page_size = 2^page_shift, or page_shift < 0
   int32_t causal, window;  // window 0: none
   int32_t workers, min_units;
+  int32_t pad;   // units that stand for an item's start and end on the line
   int32_t whole; // 1: a worker takes the items that begin in its stretch, whole; nothing is split
   int32_t rows_above, rows_upto; // sequences with rows in (rows_above, rows_upto] are this launch's
   float scale_log2;              // scale * log2(e): scores are kept in exp2 units
 };
 
-// How a kernel cuts its work (kRows, kUnit) and what an item costs beside its units (kPad, in units).
-template <int kRows_, int kUnit_, int kPad_> struct Grain {
-  static constexpr int kRows = kRows_, kUnit = kUnit_, kPad = kPad_;
+// How a kernel cuts its work.
+template <int kRows_, int kUnit_> struct Grain {
+  static constexpr int kRows = kRows_, kUnit = kUnit_;
 };
+// 64-bit quotients cost a hundred instructions; nearly all of these fit 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int32_t b) {
+  return a < (int64_t{1} << 31) ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
 struct Sequence {
   int q0, tokens, rows, kv; // first token, new tokens, tokens * group, keys
-  int blocks, first_unit, units; // row blocks; the key units that any row sees
-  int span;                      // an item's length on the line
+  int blocks, pair_span, last_span; // row blocks; the length of two paired ones on the line, and of an odd last one
+  int64_t head_span;                // of all blocks of one head
 };
+
+// The keys that row block `block` sees, [lo, hi), and the units they lie in.
+struct Keys {
+  int lo, hi, first_unit, units;
+};
+template <typename G> __device__ __forceinline__ Keys keys_of(const PagedParams &P, const Sequence &s, int block) {
+  Keys k{0, s.kv, 0, 0};
+  const int past = s.kv - s.tokens; // position of token 0 (negative: its first tokens see nothing)
+  const int row0 = block * G::kRows;
+  // (the last block ends with the sequence and the first begins with it: no quotient for a single one)
+  if (P.causal && row0 + G::kRows < s.rows) k.hi = max(0, min(s.kv, past + (row0 + G::kRows - 1) / P.group + 1));
+  if (P.window > 0) {
+    const int64_t lo = static_cast<int64_t>(past) + (block > 0 ? row0 / P.group : 0) - P.window + 1;
+    k.lo = lo > 0 ? static_cast<int>(min(lo, static_cast<int64_t>(s.kv))) : 0;
+  }
+  k.first_unit = k.lo / G::kUnit;
+  k.units = max(1, (k.hi + G::kUnit - 1) / G::kUnit - k.first_unit); // an item without keys still has its zeros to write
+  return k;
+}
 
 // The sequence's shape, with every offset forced into range (and reported when it was not).
 template <typename G> __device__ __forceinline__ Sequence sequence(const PagedParams &P, int b) {
@@ -75,24 +101,55 @@ template <typename G> __device__ __forceinline__ Sequence sequence(const PagedPa
   const int64_t rows = static_cast<int64_t>(s.tokens) * P.group;
   s.rows = rows > P.rows_above && rows <= P.rows_upto ? static_cast<int>(rows) : 0;
   s.blocks = (s.rows + G::kRows - 1) / G::kRows;
-  const int64_t first = P.window > 0 ? static_cast<int64_t>(s.kv) - s.tokens - P.window + 1 : 0;
-  s.first_unit = first > 0 ? static_cast<int>(first / G::kUnit) : 0;
-  s.units = max(1, (s.kv + G::kUnit - 1) / G::kUnit - s.first_unit); // an item without keys still has its zeros to write
-  s.span = s.units + G::kPad;
+  s.pair_span = s.last_span = 0;
+  if (s.blocks & 1) s.last_span = keys_of<G>(P, s, s.blocks - 1).units + P.pad;
+  if (s.blocks > 1) {
+    // keys grow linearly from block to block, cut off at 0: the sum of a pair is largest at the ends or in the middle,
+    // and a unit more at either end of both where they do not begin and end on units
+    const int last = (s.blocks & ~1) - 1;
+    const int ends = keys_of<G>(P, s, 0).units + keys_of<G>(P, s, last).units;
+    const int middle = keys_of<G>(P, s, last / 2).units + keys_of<G>(P, s, last / 2 + 1).units;
+    s.pair_span = max(ends, middle) + 2 + 2 * P.pad;
+  }
+  s.head_span = static_cast<int64_t>(s.blocks >> 1) * s.pair_span + s.last_span;
   return s;
 }
-template <typename G> __device__ __forceinline__ int64_t sequence_span(const PagedParams &P, int b) {
-  const Sequence s = sequence<G>(P, b);
-  return static_cast<int64_t>(s.blocks) * s.span * P.k_heads;
-}
+template <typename G> __device__ __forceinline__ int64_t sequence_span(const PagedParams &P, int b) { return sequence<G>(P, b).head_span * P.k_heads; }
 
-// Row blocks are walked from both ends (0, last, 1, last - 1, ...): under the causal mask the work of two
-// neighbours in that order adds up to the same.
-__device__ __forceinline__ int block_of(int i, int blocks) { return i & 1 ? blocks - 1 - (i >> 1) : i >> 1; }
-
-// 64-bit quotients cost a hundred instructions; nearly all of these fit 32 bits.
-__device__ __forceinline__ int64_t quotient(int64_t a, int32_t b) {
-  return a < (int64_t{1} << 31) ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+// The item at a place on the line, of a sequence that begins at `start`: its stretch of the line [begin, end), of
+// which the first keys.units are its units.
+struct Item {
+  int64_t begin, end;
+  int h, block;
+  Keys keys;
+};
+template <typename G> __device__ __forceinline__ Item item_at(const PagedParams &P, const Sequence &s, int64_t start, int64_t at) {
+  Item x;
+  const bool big = s.head_span >= (int64_t{1} << 31);
+  x.h = static_cast<int>(big ? (at - start) / s.head_span : quotient(at - start, static_cast<int32_t>(s.head_span)));
+  x.begin = start + x.h * s.head_span;
+  const int64_t inside = at - x.begin, pairs = static_cast<int64_t>(s.blocks >> 1) * s.pair_span;
+  if (inside >= pairs) {
+    x.block = s.blocks - 1;
+    x.keys = keys_of<G>(P, s, x.block);
+    x.begin += pairs;
+    x.end = x.begin + s.last_span;
+    return x;
+  }
+  const int pair = static_cast<int>(quotient(inside, s.pair_span));
+  x.begin += static_cast<int64_t>(pair) * s.pair_span;
+  x.end = x.begin + s.pair_span;
+  x.block = pair;
+  x.keys = keys_of<G>(P, s, pair);
+  const int64_t second = x.begin + x.keys.units + P.pad;
+  if (at < second) {
+    x.end = second;
+  } else {
+    x.begin = second;
+    x.block = (s.blocks & ~1) - 1 - pair;
+    x.keys = keys_of<G>(P, s, x.block);
+  }
+  return x;
 }
 
 // The whole line, dealt out evenly: worker w's stretch begins at stretch(w) (w = workers: the line's end).
@@ -176,12 +233,12 @@ template <typename G> __device__ __forceinline__ void note_split(const PagedPara
   if (w > 0 && w < line.workers) {
     const Sequence s = sequence<G>(P, b);
     const int64_t at = line.stretch(w);
-    const int64_t item = quotient(at - start, s.span); // head * blocks + place of the row block
-    const int64_t begin = start + item * s.span, end = begin + s.units;
-    if (begin < at && at < end && begin >= line.stretch(w - 1)) {
+    const Item item = item_at<G>(P, s, start, at);
+    const int64_t end = item.begin + item.keys.units;
+    if (item.begin < at && at < end && item.begin >= line.stretch(w - 1)) {
       x.q0 = s.q0;
-      x.h = static_cast<int>(quotient(item, s.blocks));
-      x.row0 = block_of(static_cast<int>(item - static_cast<int64_t>(x.h) * s.blocks), s.blocks) * G::kRows;
+      x.h = item.h;
+      x.row0 = item.block * G::kRows;
       x.rows = min(G::kRows, s.rows - x.row0);
       int last = w; // the last worker with a part
       while (last + 1 < line.workers && line.stretch(last + 1) < end) ++last;
@@ -254,7 +311,7 @@ template <int kThreads, int kRows, int kDim, typename Store> __device__ __forcei
     store(token, head, c, sum != 0.f ? v / sum : 0.f);
   }
   if (threadIdx.x == 0 && P.lse != nullptr)
-    P.lse[static_cast<int64_t>(token) * P.q_heads + head] = sum != 0.f ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+    P.lse[static_cast<int64_t>(token) * (P.k_heads * P.group) + head] = sum != 0.f ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
 }
 
 // The same for items with many rows, which have few parts: block (w - 1, y) takes the rows y * kBlockRows .. of w's
@@ -316,7 +373,7 @@ template <int kRows, int kDim, typename Store> __device__ __forceinline__ void c
     for (int c = 0; c < kPer; ++c)
       if (c * 32 + lane < P.head_dim) store(token, head, c * 32 + lane, l[i] != 0.f ? acc[i][c] / l[i] : 0.f);
     if (lane == 0 && P.lse != nullptr)
-      P.lse[static_cast<int64_t>(token) * P.q_heads + head] = l[i] != 0.f ? (m[i] + log2f(l[i])) * 0.69314718055994531f : -INFINITY;
+      P.lse[static_cast<int64_t>(token) * (P.k_heads * P.group) + head] = l[i] != 0.f ? (m[i] + log2f(l[i])) * 0.69314718055994531f : -INFINITY;
   }
 }
 

@@ -33,7 +33,7 @@ template <typename T, int kDim> struct Config {
   static constexpr int kWarps = kRowBytes <= 512 ? 4 : 2; // 3 stages of 16 keys and values per warp must fit
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kUnit = 64; // keys of a unit: the same for every type, so that the host can count
-  using Cut = khp::Grain<kRows, kUnit, 1>; // an item's start and end cost about a unit
+  using Cut = khp::Grain<kRows, kUnit>;
   static constexpr int kSteps = kUnit / (kKeys * kWarps);
   static constexpr int kPitch = kRowBytes + 16; // bytes between rows: ldmatrix and fp32 reads without bank conflicts
   static constexpr int kTile = kKeys * kPitch;
@@ -243,35 +243,33 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
   int64_t at = from, start = scratch.start;
   int b = scratch.b;
   khp::Sequence s = khp::sequence<Cut>(P, b);
-  if (P.whole) at = start + khp::quotient(at - start + s.span - 1, s.span) * s.span; // the first item that begins here
+  if (P.whole) { // the first item that begins here
+    const khp::Item item = khp::item_at<Cut>(P, s, start, at);
+    if (item.begin < at) at = item.end;
+  }
 
   const bool whole_steps = P.page_size % kKeys == 0; // a step's keys lie in one page
   const int chunks_per_row = P.head_dim * static_cast<int>(sizeof(T)) / 16; // 16-byte pieces that exist
   while (at < until) {
-    int64_t size = static_cast<int64_t>(s.blocks) * s.span * P.k_heads;
-    while (at >= start + size) { // on to the next sequence that has rows
-      start += size;
+    while (at >= start + s.head_span * P.k_heads) { // on to the next sequence that has rows
+      start += s.head_span * P.k_heads;
       s = khp::sequence<Cut>(P, ++b);
-      size = static_cast<int64_t>(s.blocks) * s.span * P.k_heads;
     }
-    const int64_t item = khp::quotient(at - start, s.span);
-    const int64_t begin = start + item * s.span, end = begin + s.span;
-    if (at - begin >= s.units) { // what is left of the item is only what stands for its end
-      at = end;
+    const khp::Item item = khp::item_at<Cut>(P, s, start, at);
+    if (at - item.begin >= item.keys.units) { // what is left of the item is only what stands for its end
+      at = item.end;
       continue;
     }
-    const int h = static_cast<int>(khp::quotient(item, s.blocks));
-    const int block = khp::block_of(static_cast<int>(item - static_cast<int64_t>(h) * s.blocks), s.blocks);
-    const int unit0 = static_cast<int>(at - begin), unit1 = P.whole ? s.units : static_cast<int>(min((until < end ? until : end) - begin, static_cast<int64_t>(s.units)));
-    const int row0 = block * kRows, rows_here = min(kRows, s.rows - row0);
-    // keys that rows of this block see, and the part of them in this stretch
+    const int h = item.h;
+    const int unit0 = static_cast<int>(at - item.begin);
+    const int unit1 = P.whole ? item.keys.units : static_cast<int>(min((until < item.end ? until : item.end) - item.begin, static_cast<int64_t>(item.keys.units)));
+    const int row0 = item.block * kRows, rows_here = min(kRows, s.rows - row0);
     const int t_first = row0 / P.group, t_last = (row0 + rows_here - 1) / P.group;
     const int past = s.kv - s.tokens; // position of token 0 (negative: its first tokens see nothing)
-    const int hi_key = P.causal ? max(0, min(s.kv, past + t_last + 1)) : s.kv;
-    const int64_t lo_window = P.window > 0 ? static_cast<int64_t>(past) + t_first - P.window + 1 : 0;
-    const int lo_key = lo_window > 0 ? static_cast<int>(min(lo_window, static_cast<int64_t>(s.kv))) : 0;
-    const int key_a = max((s.first_unit + unit0) * kUnit, lo_key / kUnit * kUnit);
-    const int key_b = static_cast<int>(min(static_cast<int64_t>(s.first_unit + unit1) * kUnit, static_cast<int64_t>(hi_key)));
+    // keys that rows of this block see, in this stretch
+    const int lo_key = item.keys.lo;
+    const int key_a = (item.keys.first_unit + unit0) * kUnit;
+    const int key_b = static_cast<int>(min(static_cast<int64_t>(item.keys.first_unit + unit1) * kUnit, static_cast<int64_t>(item.keys.hi)));
 
     // this lane's two rows: their queries and the keys they see
     const int g = lane >> 2;
@@ -456,8 +454,8 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
         *reinterpret_cast<float2 *>(mine + (g + 8 * i2) * kPitchF + n * 8 + 2 * (lane & 3)) = make_float2(o[n][2 * i2] * f, o[n][2 * i2 + 1] * f);
     }
     __syncthreads();
-    const bool whole = unit0 == 0 && unit1 == s.units;
-    const int64_t part = begin < from ? 2 * static_cast<int64_t>(w) : 2 * static_cast<int64_t>(w) + 1;
+    const bool whole = unit0 == 0 && unit1 == item.keys.units;
+    const int64_t part = item.begin < from ? 2 * static_cast<int64_t>(w) : 2 * static_cast<int64_t>(w) + 1;
     for (int i = threadIdx.x; i < rows_here * (kDim / 4); i += kThreads) {
       const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
       float top = s_m[0][r];
@@ -486,14 +484,14 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
         else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]));
       }
       if (c == 0 && P.lse != nullptr)
-        P.lse[static_cast<int64_t>(s.q0 + t) * P.q_heads + head] = sum != 0.f ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+        P.lse[static_cast<int64_t>(s.q0 + t) * (P.k_heads * P.group) + head] = sum != 0.f ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
     }
     __syncthreads(); // the scratch becomes rings again
     if (P.head_dim < kDim) { // and their unwritten columns zeros
       for (int i = threadIdx.x * 16; i < kWarps * Cfg::kRing; i += kThreads * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
       __syncthreads();
     }
-    at = until < end && !P.whole ? until : end;
+    at = until < item.end && !P.whole ? until : item.end;
   }
   if (threadIdx.x == 0 && !P.whole) khp::note_split<Cut>(P, line, w, scratch.b, scratch.start);
 }

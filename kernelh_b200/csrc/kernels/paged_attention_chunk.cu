@@ -9,7 +9,7 @@
 //
 // One block per SM, 16 warps. Warpgroups 0 and 1, a thread per row, are the softmax of the two tiles; while one
 // works, the tensor core does the other tile's P V and the next Q K^T, so the two keep it busy in turns. Warp 8
-// issues the matrix instructions, warp 10 the copies, warps 12 to 15 bring in the queries of the next item while this
+// issues the matrix instructions, warp 9 the copies, warp 10 works out the items, warps 12 to 15 bring in the queries of the next item while this
 // one's last tile is worked on. The boxes of a tile of keys are looked up in the page table by one
 // lane each and fetched by TMA straight out of the pages (a box is the largest power of two of slots that divides
 // the page, so none crosses a page), keys and values through one ring. Pages therefore cost nothing but the
@@ -43,10 +43,10 @@ using khp::PagedParams;
 constexpr int kTileRows = 128;
 constexpr int kRows = 2 * kTileRows; // rows of an item
 constexpr int kKeys = 128;           // keys of a tile
-using Cut = khp::Grain<kRows, kKeys, 3>; // an item's queries, first scores and output cost about three tiles
+using Cut = khp::Grain<kRows, kKeys>;
 constexpr int kThreads = 512;
 constexpr int kMaxStages = 8;
-constexpr int kIssueWarp = 8, kLoadWarp = 10, kQueryWarp = 12, kQueryWarps = 4;
+constexpr int kIssueWarp = 8, kLoadWarp = 9, kPlanWarp = 10, kQueryWarp = 12, kQueryWarps = 4;
 // registers after the warpgroups have traded them: two softmax groups, control, idle; 4 x 128 at launch
 constexpr int kRegsSoftmax = 200, kRegsControl = 56;
 constexpr float kLazy = 8.f;
@@ -131,53 +131,56 @@ template <> struct Types<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
 };
 
-// A worker's stretch of the line, item by item; every role walks it on its own.
-struct Work {
-  khp::Sequence s;
-  int b, h, row0, rows;  // rows: those of this item, up to 256
-  int key_a, key_b;      // its keys in this stretch: [key_a, key_b), key_a on a tile
-  int key_lo;            // the first key that any row sees (inside the first tile)
-  int tiles;
-  int64_t part;          // where a partial result goes, or -1 when the item is whole
+// A worker's part of an item.
+struct alignas(16) Work {
+  int q0, tokens, kv; // the sequence: first token, new tokens, keys
+  int b, h, row0, rows; // rows: those of this item, up to 256
+  int key_a, key_b;     // its keys in this stretch: [key_a, key_b), key_a on a tile
+  int key_lo;           // the first key that any row sees
+  int tiles;            // of keys; -1: nothing is left to do
+  int part;             // the slot of a partial result, or -1 when the item is whole
 };
+// The worker's stretch of the line, item by item. Finding the next one is a few hundred dependent instructions, 4 us:
+// one warp does it ahead of all others and hands it out through a short queue in shared memory.
 struct Walker {
   int64_t at, until, from, start;
   int b, w;
-  __device__ __forceinline__ bool next(const PagedParams &P, Work &k) {
-    int64_t item, begin, end;
+  __device__ __forceinline__ void next(const PagedParams &P, Work &k) {
+    khp::Item item;
+    khp::Sequence s;
     for (;;) {
-      if (at >= until) return false;
-      k.s = khp::sequence<Cut>(P, b);
-      int64_t size = static_cast<int64_t>(k.s.blocks) * k.s.span * P.k_heads;
-      while (at >= start + size) {
-        start += size;
-        k.s = khp::sequence<Cut>(P, ++b);
-        size = static_cast<int64_t>(k.s.blocks) * k.s.span * P.k_heads;
+      if (at >= until) {
+        k.tiles = -1;
+        return;
       }
-      item = khp::quotient(at - start, k.s.span);
-      begin = start + item * k.s.span, end = begin + k.s.span;
-      if (at - begin < k.s.units) break;
-      at = end; // what is left of the item is only what stands for its end
+      s = khp::sequence<Cut>(P, b);
+      while (at >= start + s.head_span * P.k_heads) {
+        start += s.head_span * P.k_heads;
+        s = khp::sequence<Cut>(P, ++b);
+      }
+      item = khp::item_at<Cut>(P, s, start, at);
+      if (at - item.begin < item.keys.units) break;
+      at = item.end; // what is left of the item is only what stands for its end
     }
+    const int unit0 = static_cast<int>(at - item.begin);
+    const int unit1 = static_cast<int>(min((until < item.end ? until : item.end) - item.begin, static_cast<int64_t>(item.keys.units)));
+    k.q0 = s.q0;
+    k.tokens = s.tokens;
+    k.kv = s.kv;
     k.b = b;
-    k.h = static_cast<int>(khp::quotient(item, k.s.blocks));
-    const int block = khp::block_of(static_cast<int>(item - static_cast<int64_t>(k.h) * k.s.blocks), k.s.blocks);
-    const int unit0 = static_cast<int>(at - begin), unit1 = static_cast<int>(min((until < end ? until : end) - begin, static_cast<int64_t>(k.s.units)));
-    k.row0 = block * kRows;
-    k.rows = min(kRows, k.s.rows - k.row0);
-    const int t_first = k.row0 / P.group, t_last = (k.row0 + k.rows - 1) / P.group;
-    const int past = k.s.kv - k.s.tokens;
-    const int hi = P.causal ? max(0, min(k.s.kv, past + t_last + 1)) : k.s.kv;
-    const int64_t lo_window = P.window > 0 ? static_cast<int64_t>(past) + t_first - P.window + 1 : 0;
-    k.key_lo = lo_window > 0 ? static_cast<int>(min(lo_window, static_cast<int64_t>(k.s.kv))) : 0;
-    k.key_a = max((k.s.first_unit + unit0) * kKeys, k.key_lo / kKeys * kKeys);
-    k.key_b = static_cast<int>(min(static_cast<int64_t>(k.s.first_unit + unit1) * kKeys, static_cast<int64_t>(hi)));
+    k.h = item.h;
+    k.row0 = item.block * kRows;
+    k.rows = min(kRows, s.rows - k.row0);
+    k.key_lo = item.keys.lo;
+    k.key_a = (item.keys.first_unit + unit0) * kKeys;
+    k.key_b = static_cast<int>(min(static_cast<int64_t>(item.keys.first_unit + unit1) * kKeys, static_cast<int64_t>(item.keys.hi)));
     k.tiles = k.key_b > k.key_a ? (k.key_b - k.key_a + kKeys - 1) / kKeys : 0;
-    k.part = unit0 == 0 && unit1 == k.s.units ? -1 : (begin < from ? 2 * static_cast<int64_t>(w) : 2 * static_cast<int64_t>(w) + 1);
-    at = until < end ? until : end;
-    return true;
+    k.part = unit0 == 0 && unit1 == item.keys.units ? -1 : (item.begin < from ? 2 * w : 2 * w + 1);
+    at = until < item.end ? until : item.end;
   }
 };
+constexpr int kQueue = 4;
+constexpr int kReaders = 8 + 1 + 1 + kQueryWarps; // warps that take every item
 
 template <typename T, int kDim>
 __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::TensorMap &tm_k, const khd::TensorMap &tm_v, int box_rows) {
@@ -186,7 +189,8 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
   constexpr uint32_t kHalfBytes = kKeys * 128; // 128 rows of 128 bytes
   constexpr int kStages = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[10 + 2 * kMaxStages];
+  __shared__ __align__(8) uint64_t bars[10 + 2 * kMaxStages + 2 * kQueue];
+  __shared__ Work s_work[kQueue];
   __shared__ khp::LineScratch<kThreads> scratch;
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
@@ -196,7 +200,8 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
   const uint32_t smem_ring = smem_q + 2 * Cfg::kTileBytes;
   const uint32_t bar_q = khd::smem_u32(&bars[0]), bar_s = khd::smem_u32(&bars[2]), bar_p = khd::smem_u32(&bars[4]),
                  bar_o = khd::smem_u32(&bars[6]), bar_q_free = khd::smem_u32(&bars[8]), bar_full = khd::smem_u32(&bars[10]),
-                 bar_empty = khd::smem_u32(&bars[10 + kMaxStages]);
+                 bar_empty = khd::smem_u32(&bars[10 + kMaxStages]), bar_work = khd::smem_u32(&bars[10 + 2 * kMaxStages]),
+                 bar_taken = khd::smem_u32(&bars[10 + 2 * kMaxStages + kQueue]);
   if (threadIdx.x == 0) {
     s_abort = 0;
     for (int g = 0; g < 2; ++g) {
@@ -209,6 +214,10 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
     for (int i = 0; i < kStages; ++i) {
       khd::mbar_init(bar_full + 8 * i, 1);
       khd::mbar_init(bar_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < kQueue; ++i) {
+      khd::mbar_init(bar_work + 8 * i, 1);
+      khd::mbar_init(bar_taken + 8 * i, kReaders);
     }
     khd::mbar_fence_init();
     khd::tma_prefetch_descriptor(&tm_k);
@@ -226,25 +235,52 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
   khd::grid_dependents_may_launch();
 
   const khp::Line line = khp::lay_line<kThreads, Cut>(P, blockIdx.x, scratch);
-  Walker walker{};
-  walker.w = blockIdx.x;
-  if (walker.w < line.workers) {
-    walker.from = walker.at = line.stretch(walker.w);
-    walker.until = line.stretch(walker.w + 1);
-    walker.b = scratch.b;
-    walker.start = scratch.start;
-  }
-  if (threadIdx.x == kThreads - 1) khp::note_split<Cut>(P, line, walker.w, walker.b, walker.start);
+  // The next item of the queue, for a whole warp; false when there is none or a wait ran out.
   Work k;
+  uint32_t work_count = 0;
+  const auto take = [&] {
+    const uint32_t i = work_count % kQueue;
+    const bool ready = khd::mbar_wait(bar_work + 8 * i, (work_count / kQueue) & 1u, &s_abort, P.status, khd::kStatusEmptyWaitTimeout, 6900u);
+    if (!__all_sync(0xffffffffu, ready)) return false;
+    k = s_work[i];
+    warp_arrive(bar_taken + 8 * i);
+    ++work_count;
+    return k.tiles >= 0;
+  };
 
   if (warp >= 8) {
     registers_release<kRegsControl>();
-    if (warp == kLoadWarp) {
+    if (warp == kPlanWarp) {
+      // ---- the worker's items, in turn, ahead of everybody ------------------------------------------------------
+      Walker walker{};
+      walker.w = blockIdx.x;
+      if (walker.w < line.workers) {
+        walker.from = walker.at = line.stretch(walker.w);
+        walker.until = line.stretch(walker.w + 1);
+        walker.b = scratch.b;
+        walker.start = scratch.start;
+      }
+      const int first_b = walker.b;
+      const int64_t first_start = walker.start;
+      for (uint32_t n = 0;; ++n) {
+        const uint32_t i = n % kQueue;
+        walker.next(P, k);
+        const bool ready = khd::mbar_wait(bar_taken + 8 * i, ((n / kQueue) & 1u) ^ 1u, &s_abort, P.status, khd::kStatusEmptyWaitTimeout, 6950u);
+        if (!__all_sync(0xffffffffu, ready)) break;
+        if (lane == 0) {
+          s_work[i] = k;
+          khd::mbar_arrive(bar_work + 8 * i);
+        }
+        __syncwarp();
+        if (k.tiles < 0) break;
+      }
+      if (lane == 0) khp::note_split<Cut>(P, line, walker.w, first_b, first_start);
+    } else if (warp == kLoadWarp) {
       // ---- copies: K and V tiles of every item in turn through the ring. Lane i looks up and fetches box i. ----
       uint32_t slot = 0, phase = 0;
       bool ok = true;
       const int boxes = kKeys / box_rows;
-      while (ok && walker.next(P, k)) {
+      while (ok && take()) {
         const int32_t *table = P.table + k.b * P.table_stride;
         for (int j = 0; j < k.tiles && ok; ++j) {
           const int key = k.key_a + j * kKeys + lane * box_rows; // of this lane's box
@@ -315,7 +351,7 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
         }
         __syncwarp();
       };
-      while (ok && __any_sync(0xffffffffu, walker.next(P, k))) {
+      while (ok && take()) {
         const int tiles = __shfl_sync(0xffffffffu, k.tiles, 0), groups = __shfl_sync(0xffffffffu, k.rows, 0) > kTileRows ? 2 : 1;
         const int key_a = __shfl_sync(0xffffffffu, k.key_a, 0), key_b = __shfl_sync(0xffffffffu, k.key_b, 0),
                   key_lo = __shfl_sync(0xffffffffu, k.key_lo, 0);
@@ -380,7 +416,7 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
       //      row x lies at chunk c ^ (x % 8) of its 128 bytes (the swizzle a TMA copy would have written). ----
       uint32_t phase[2] = {1, 1};
       bool ok = true;
-      while (ok && walker.next(P, k)) {
+      while (ok && take()) {
         if (k.tiles == 0) continue;
         for (int g = 0; g < 2 && g * kTileRows < k.rows && ok; ++g) {
           ok = khd::mbar_wait(bar_q_free + 8 * g, phase[g], &s_abort, P.status, khd::kStatusEmptyWaitTimeout, 6800u);
@@ -393,7 +429,7 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
             const int idx = (i * kQueryWarps + warp - kQueryWarp) * 32 + lane, x = idx / kChunks, c = idx % kChunks;
             const bool real = g * kTileRows + x < k.rows && c * 8 < P.head_dim;
             const int qr = k.row0 + (real ? g * kTileRows + x : 0), qt = qr / P.group;
-            const T *src = reinterpret_cast<const T *>(P.q) + (k.s.q0 + qt) * P.q_token + (k.h * P.group + qr - qt * P.group) * P.q_head +
+            const T *src = reinterpret_cast<const T *>(P.q) + (k.q0 + qt) * P.q_token + (k.h * P.group + qr - qt * P.group) * P.q_head +
                            (real ? c * 8 : 0);
             const uint32_t dst = smem_q + g * Cfg::kTileBytes + (c >> 3) * kHalfBytes + x * 128 + (((c & 7) ^ (x & 7)) << 4);
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
@@ -413,16 +449,16 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
     const uint32_t t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
     uint32_t s_phase = 0, o_phase = 0;
     bool ok = true;
-    while (ok && walker.next(P, k)) {
+    while (ok && take()) {
       const int rows_here = k.rows - g * kTileRows; // of this tile
       if (rows_here <= 0) continue;
       const int r = k.row0 + g * kTileRows + row;
       const bool real = row < rows_here;
       const int t = real ? r / P.group : 0, head = k.h * P.group + (real ? r - t * P.group : 0);
-      const int past = k.s.kv - k.s.tokens;
-      const int see_hi = !real ? -1 : P.causal ? past + t : k.s.kv - 1;
+      const int past = k.kv - k.tokens;
+      const int see_hi = !real ? -1 : P.causal ? past + t : k.kv - 1;
       const int64_t first = P.window > 0 ? static_cast<int64_t>(past) + t - P.window + 1 : 0;
-      const int see_lo = first > 0 ? static_cast<int>(min(first, static_cast<int64_t>(k.s.kv))) : 0;
+      const int see_lo = first > 0 ? static_cast<int>(min(first, static_cast<int64_t>(k.kv))) : 0;
       const bool idle = quad * 32 >= rows_here; // no row of this warp is real: its lanes of P may hold anything
       float m = -INFINITY, l = 0.f;             // reference and sum, in exp2 units
       for (int j = 0; j < k.tiles; ++j) {
@@ -497,8 +533,8 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
       }
       if (!idle) {
         const float inv = l != 0.f ? 1.f / l : 0.f; // a row that sees no key: zeros
-        const int64_t at = k.part * kRows + g * kTileRows + row;
-        T *dst = reinterpret_cast<T *>(P.o) + (k.s.q0 + t) * P.o_token + head * P.o_head;
+        const int64_t at = static_cast<int64_t>(k.part) * kRows + g * kTileRows + row;
+        T *dst = reinterpret_cast<T *>(P.o) + (k.q0 + t) * P.o_token + head * P.o_head;
 #pragma unroll
         for (int i = 0; i < kDim / 32; ++i) {
           uint32_t o[32];
@@ -529,7 +565,7 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
         if (real) {
           if (k.part >= 0) P.partial_ml[at] = make_float2(m, l);
           else if (P.lse != nullptr)
-            P.lse[static_cast<int64_t>(k.s.q0 + t) * P.q_heads + head] = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+            P.lse[static_cast<int64_t>(k.q0 + t) * (P.k_heads * P.group) + head] = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
         }
       }
     }

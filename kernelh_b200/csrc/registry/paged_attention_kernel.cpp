@@ -36,9 +36,9 @@ struct PagedParams {
   float *lse, *partial_o;
   void *partial_ml, *split_items;
   uint32_t *status;
-  int32_t tokens, batch, q_heads, k_heads, group, head_dim, page_size, page_shift, table_width, num_pages;
+  int32_t tokens, batch, k_heads, group, head_dim, page_size, page_shift, table_width, num_pages;
   int32_t causal, window;
-  int32_t workers, min_units, whole;
+  int32_t workers, min_units, pad, whole;
   int32_t rows_above, rows_upto;
   float scale_log2;
 };
@@ -169,7 +169,7 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
   p.lse = a.lse;
   p.partial_o = static_cast<float *>(a.workspace);
   p.status = ex.status_word();
-  p.tokens = static_cast<int32_t>(a.tokens), p.batch = a.batch, p.q_heads = a.q_heads, p.k_heads = a.k_heads;
+  p.tokens = static_cast<int32_t>(a.tokens), p.batch = a.batch, p.k_heads = a.k_heads;
   p.group = a.q_heads / a.k_heads, p.head_dim = a.head_dim;
   p.page_size = a.page_size, p.page_shift = (a.page_size & (a.page_size - 1)) == 0 ? std::countr_zero(static_cast<unsigned>(a.page_size)) : -1;
   p.table_width = a.table_width, p.num_pages = static_cast<int32_t>(a.num_pages);
@@ -197,6 +197,11 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
   const auto workers = [&](int rows, int unit, int per_sm) {
     const int64_t n = worker_count(a, rows, unit, per_sm, sms);
     p.workers = static_cast<int32_t>(n);
+    // An item's start and end take about as long as four units of 128 keys and 256 rows, or three of 64 and 16. Where
+    // items are fewer than workers, each is worked on by several, and units that stand for nothing would only leave
+    // some of these without work. (64 ragged decoding sequences 200 us with 1, 172 with 3; 8 fp32 ones, 128 items,
+    // 20.8 with 1, 24.2 with 3; 13 mixed ones 210 us in the chunk kernel with 0, 130 with 3 or 4.)
+    p.pad = (rows == kChunkRows ? 2 : 1) + (item_count(a, rows) >= n ? 2 : 0);
     char *base = static_cast<char *>(a.workspace); // rows, notes of split items, (max, sum) pairs
     p.split_items = base + 2 * n * rows * s.dim * 4;
     p.partial_ml = base + 2 * n * rows * s.dim * 4 + n * 32;
@@ -206,9 +211,11 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
   p.rows_above = 0, p.rows_upto = INT_MAX;
 
   if (many_rows(a) && chunk_kernel_fits(a)) {
-    // A sequence of at most 16 rows (a decoding one) goes to the other kernel, unless there can be none: when the
-    // longest length times the batch is no more than the tokens, every sequence has that length.
-    const bool alone = static_cast<int64_t>(a.batch) * a.max_q_len <= a.tokens;
+    // A sequence of at most 16 rows (a decoding one) goes to the other kernel, unless there can be none (when the
+    // longest length times the batch is no more than the tokens, every sequence has that length), or so few that
+    // they cost less among the chunks than two more launches: 13 sequences, 8 of them decoding, 155 us against 166 with
+    // both kernels, but 32 of up to 8 tokens 170 against 150 (8 key/value heads).
+    const bool alone = static_cast<int64_t>(a.batch) * a.max_q_len <= a.tokens || static_cast<int64_t>(a.batch) * a.k_heads <= sms;
     if (!alone) p.rows_above = kRows;
     int box_rows = kChunkKeys; // the largest power of two of slots that divides a page and a tile
     while (a.page_size % box_rows != 0) box_rows /= 2;
