@@ -227,23 +227,20 @@ struct alignas(32) SplitItem {
   int32_t q0, row0, rows, h, parts; // rows: of the item
 };
 __device__ __forceinline__ int64_t part_slot(int w, int p) { return 2 * static_cast<int64_t>(w - 1 + p) + (p == 0 ? 1 : 0); }
-// One thread of worker w notes it down. The stretch begins in sequence b, which begins at `start`.
-template <typename G> __device__ __forceinline__ void note_split(const PagedParams &P, const Line &line, int w, int b, int64_t start) {
+// One thread of worker w notes it down; `item` (of sequence s) is where its stretch begins.
+template <typename G> __device__ __forceinline__ void note_split(const PagedParams &P, const Line &line, int w, const Sequence &s, const Item &item) {
   SplitItem x{};
-  if (w > 0 && w < line.workers) {
-    const Sequence s = sequence<G>(P, b);
-    const int64_t at = line.stretch(w);
-    const Item item = item_at<G>(P, s, start, at);
-    const int64_t end = item.begin + item.keys.units;
-    if (item.begin < at && at < end && item.begin >= line.stretch(w - 1)) {
-      x.q0 = s.q0;
-      x.h = item.h;
-      x.row0 = item.block * G::kRows;
-      x.rows = min(G::kRows, s.rows - x.row0);
-      int last = w; // the last worker with a part
-      while (last + 1 < line.workers && line.stretch(last + 1) < end) ++last;
-      x.parts = last - w + 2;
-    }
+  const int64_t at = line.stretch(w), end = item.begin + item.keys.units;
+  if (item.begin < at && at < end && item.begin >= line.stretch(w - 1)) {
+    x.q0 = s.q0;
+    x.h = item.h;
+    x.row0 = item.block * G::kRows;
+    x.rows = min(G::kRows, s.rows - x.row0);
+    // the last worker with a part: by proportion, then to the place
+    int last = max(w, min(line.workers - 1, static_cast<int>((end - 1) * line.workers / line.total)));
+    while (last + 1 < line.workers && line.stretch(last + 1) < end) ++last;
+    while (last > w && line.stretch(last) >= end) --last;
+    x.parts = last - w + 2;
   }
   P.split_items[w] = x;
 }

@@ -257,6 +257,7 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
     }
     const khp::Item item = khp::item_at<Cut>(P, s, start, at);
     if (at - item.begin >= item.keys.units) { // what is left of the item is only what stands for its end
+      if (threadIdx.x == 0 && at == from && !P.whole) P.split_items[w] = khp::SplitItem{};
       at = item.end;
       continue;
     }
@@ -366,6 +367,7 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
     look_up(0);
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i);
+    if (threadIdx.x == 0 && at == from && !P.whole) khp::note_split<Cut>(P, line, w, s, item); // while the first copies fly
     for (int i = 0; i < steps; ++i) {
       __syncwarp(); // every lane is done with the slot that is refilled now
       issue(i + kStages - 1);
@@ -493,7 +495,6 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
     }
     at = until < item.end && !P.whole ? until : item.end;
   }
-  if (threadIdx.x == 0 && !P.whole) khp::note_split<Cut>(P, line, w, scratch.b, scratch.start);
 }
 
 template <typename T, int kDim> __device__ __forceinline__ void combine(const PagedParams &P) {

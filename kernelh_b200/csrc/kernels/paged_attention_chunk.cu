@@ -260,8 +260,6 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
         walker.b = scratch.b;
         walker.start = scratch.start;
       }
-      const int first_b = walker.b;
-      const int64_t first_start = walker.start;
       for (uint32_t n = 0;; ++n) {
         const uint32_t i = n % kQueue;
         walker.next(P, k);
@@ -274,7 +272,14 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
         __syncwarp();
         if (k.tiles < 0) break;
       }
-      if (lane == 0) khp::note_split<Cut>(P, line, walker.w, first_b, first_start);
+      if (lane == 0) {
+        if (walker.w < line.workers) {
+          const khp::Sequence s = khp::sequence<Cut>(P, scratch.b);
+          khp::note_split<Cut>(P, line, walker.w, s, khp::item_at<Cut>(P, s, scratch.start, walker.from));
+        } else {
+          P.split_items[walker.w] = khp::SplitItem{};
+        }
+      }
     } else if (warp == kLoadWarp) {
       // ---- copies: K and V tiles of every item in turn through the ring. Lane i looks up and fetches box i. ----
       uint32_t slot = 0, phase = 0;
