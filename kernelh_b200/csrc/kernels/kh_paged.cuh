@@ -104,12 +104,14 @@ template <typename G> __device__ __forceinline__ Sequence sequence(const PagedPa
   s.pair_span = s.last_span = 0;
   if (s.blocks & 1) s.last_span = keys_of<G>(P, s, s.blocks - 1).units + P.pad;
   if (s.blocks > 1) {
-    // keys grow linearly from block to block, cut off at 0: the sum of a pair is largest at the ends or in the middle,
-    // and a unit more at either end of both where they do not begin and end on units
+    // No pair may be longer than pair_span. The last key a block sees grows linearly from block to block (cut off at 0,
+    // which makes the sum of a pair largest at the ends), so does the first one under a window (cut off at 0, with the
+    // opposite sign: largest in the middle). Either pair may be rounded up to units by two less than another is, by
+    // four with a window, and the one at the ends may be short of a block's tokens, two units at most.
     const int last = (s.blocks & ~1) - 1;
     const int ends = keys_of<G>(P, s, 0).units + keys_of<G>(P, s, last).units;
     const int middle = keys_of<G>(P, s, last / 2).units + keys_of<G>(P, s, last / 2 + 1).units;
-    s.pair_span = max(ends, middle) + 2 + 2 * P.pad;
+    s.pair_span = max(ends, middle) + (P.window > 0 ? 6 : 2) + 2 * P.pad;
   }
   s.head_span = static_cast<int64_t>(s.blocks >> 1) * s.pair_span + s.last_span;
   return s;

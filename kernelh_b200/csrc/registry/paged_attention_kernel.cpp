@@ -117,7 +117,7 @@ Result<void> check_paged_attention(const kh_paged_attention_args &a) {
                   std::to_string(a.k_heads) + ")");
   if (a.head_dim < 8 || a.head_dim > 256 || a.head_dim % 8 != 0)
     return refuse("head_dim must be a multiple of 8 up to 256 (got " + std::to_string(a.head_dim) + ")");
-  if (a.tokens < 0 || a.tokens * (a.q_heads / a.k_heads) > INT_MAX - 1024)
+  if (a.tokens < 0 || a.tokens > (INT_MAX - 1024) / (a.q_heads / a.k_heads))
     return refuse("tokens * q_heads / k_heads must lie in 0 .. 2^31 - 1025");
   if (a.batch < 0 || a.max_q_len < 0 || a.max_kv_len < 0) return refuse("batch, max_q_len and max_kv_len must not be negative");
   if (a.causal != 0 && a.causal != 1) return refuse("causal must be 0 or 1");

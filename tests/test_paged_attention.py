@@ -35,7 +35,7 @@ def call(**over):
 @pytest.mark.parametrize("over,words", [
     (dict(dtype=3), "dtype must be"), (dict(q_heads=7), "multiple of k_heads"), (dict(k_heads=0), "multiple of k_heads"),
     (dict(head_dim=60), "head_dim must be a multiple of 8"), (dict(head_dim=264), "head_dim must be a multiple of 8"),
-    (dict(tokens=-1), "tokens * q_heads"), (dict(tokens=1 << 30), "tokens * q_heads"), (dict(batch=-1), "must not be negative"),
+    (dict(tokens=-1), "tokens * q_heads"), (dict(tokens=1 << 30), "tokens * q_heads"), (dict(tokens=1 << 62), "tokens * q_heads"), (dict(batch=-1), "must not be negative"),
     (dict(causal=2), "causal"), (dict(window=-1), "window"), (dict(scale=math.inf), "scale"), (dict(scale=math.nan), "scale"),
     (dict(num_pages=0), "num_pages"), (dict(page_size=0), "page_size"), (dict(table_width=1 << 28), "page table row"),
     (dict(table_stride=6), "rows of the page table overlap"), (dict(q=(0, 512, 64)), "buffer 'q' is null"),
@@ -187,7 +187,13 @@ CASES = [  # dtype, q heads, k heads, head_dim, page, lengths, heads first, opti
     ("bf16", 8, 1, 128, 64, [(1, 40001)], False, {}), ("f32", 4, 1, 64, 16, [(2, 20011)], True, {}),
     ("f16", 32, 8, 64, 16, [(1, 1 + 37 * b % 230) for b in range(300)], False, {}),
     ("bf16", 8, 2, 128, 16, [(300, 2300), (1, 700), (1000, 1000), (17, 17)], False, {}),
-    ("bf16", 2, 2, 64, 16, [(1, 77), (4, 4)], False, dict(scale=-0.3)), ("f16", 2, 1, 64, 16, [(3, 77)], False, dict(scale=1e-30)),
+    # more sequences than a block has threads, chunks and single tokens; pages larger than a tile; one head each
+    ("bf16", 4, 4, 64, 16, [(1 + 29 * (b % 9 == 4), 40 + 31 * b % 190) for b in range(700)], False, {}),
+    ("f16", 2, 1, 128, 256, [(300, 1000), (129, 129), (2, 600)], True, {}), ("bf16", 1, 1, 64, 128, [(1500, 1500), (700, 900)], False, {}),
+    ("bf16", 3, 3, 72, 32, [(1400, 1500)], False, dict(window=333)), ("f32", 1, 1, 64, 16, [(900, 1000), (333, 300)], False, dict(window=90)),
+    # a window that is larger than the sequence, with the first queries before the first key
+    ("f16", 2, 2, 64, 8, [(700, 500), (40, 900)], False, dict(window=600)),
+    ("bf16", 2, 2, 64, 16, [(1, 77), (4, 4)], False, dict(scale=-0.3)), ("bf16", 8, 2, 128, 16, [(40, 77), (40, 40)], False, dict(scale=0.0)), ("f16", 2, 1, 64, 16, [(3, 77)], False, dict(scale=1e-30)),
 ]
 
 
