@@ -408,7 +408,7 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
       if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
 #pragma unroll
         for (int i2 = 0; i2 < 2; ++i2) {
-          const float m_new = fmaxf(m[i2], top[i2]);
+          const float m_new = top[i2] > m[i2] + kLazy ? top[i2] : m[i2]; // (a row's own: it does not depend on its neighbours)
           const float f = khd::exp2_approx(m[i2] - (m_new == -INFINITY ? 0.f : m_new));
           m[i2] = m_new;
           l[i2] *= f;

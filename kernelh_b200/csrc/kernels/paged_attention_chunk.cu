@@ -29,7 +29,7 @@
 // exponentials 400, without any softmax 365 (the products of a tile follow one another through four barriers).
 // Measured and dropped: P handed over in two (447) or four (549) parts, an issuing warp per tile (445), 2 or 3 of 8
 // exponentials by a polynomial on the multiply-add pipes (469, 490), two threads per row (556), the row maximum as a
-// thread's first score (no change: 490 against 487 at the time).
+// thread's first score (no change: 490 against 487 at the time), output rows stored by four lanes each (no change).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -490,8 +490,9 @@ __device__ __forceinline__ void chunk_body(const PagedParams &P, const khd::Tens
 #pragma unroll
             for (int x = 0; x < 4; ++x) top4[x] = max3_nan(top4[x], __uint_as_float(s[i + 2 * x]), __uint_as_float(s[i + 2 * x + 1]));
           const float top = max3_nan(max3_nan(top4[0], top4[1], top4[2]), top4[3], -INFINITY) * P.scale_log2;
-          if (__any_sync(0xffffffffu, !(top <= m + kLazy))) { // true of a NaN, which stays in m
-            const float m_new = max3_nan(m, top, -INFINITY), ref = m_new == -INFINITY ? 0.f : m_new;
+          const bool raise = !(top <= m + kLazy); // true of a NaN, which stays in m
+          if (__any_sync(0xffffffffu, raise)) {   // (a row's own reference: its result does not depend on its neighbours)
+            const float m_new = raise ? max3_nan(m, top, -INFINITY) : m, ref = m_new == -INFINITY ? 0.f : m_new;
             const float f = khd::exp2_approx(m - ref);
             m = m_new;
             l *= f;

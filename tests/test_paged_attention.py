@@ -220,6 +220,26 @@ def test_large_scores(ctx, dtype, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d,n", [("bf16", 128, 40), ("f32", 64, 40), ("f16", 256, 40), ("bf16", 64, 3)])
+def test_a_nan_stays_with_those_who_see_it(ctx, dtype, d, n):
+    """A NaN in one query row stays in it; one in a key reaches the queries that see the key and no other, nor any other
+    sequence."""
+    p = Problem(dtype, 2, 2, d, 16, [(n, 300), (n, 200)], seed=13)
+    p.run(ctx)
+    want, want_lse = p.o.clone(), p.lse.clone()
+    p.q[1, 1, 5] = math.nan
+    bad = 300 - n + 2  # seen by the queries 2 .. n - 1 of the first sequence
+    p.k[p.table[0, bad // 16].item(), bad % 16, 0, 7] = math.nan
+    p.run(ctx)
+    ctx.synchronize(stream())
+    hit = torch.zeros(p.q.shape[:2], dtype=torch.bool, device="cuda")
+    hit[1, 1] = True
+    hit[2:n, 0] = True
+    assert p.o[hit].isnan().all() and p.lse[hit].isnan().all()
+    assert torch.equal(p.o[~hit], want[~hit]) and torch.equal(p.lse[~hit], want_lse[~hit])
+
+
+@pytest.mark.gpu
 def test_lengths_beyond_the_hints(ctx):
     for dtype in ("bf16", "f32"):
         p = Problem(dtype, 8, 2, 128, 16, [(300, 900), (1, 1500)], seed=6)
