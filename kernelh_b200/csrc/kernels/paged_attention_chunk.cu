@@ -29,7 +29,9 @@
 // exponentials 400, without any softmax 365 (the products of a tile follow one another through four barriers).
 // Measured and dropped: P handed over in two (447) or four (549) parts, an issuing warp per tile (445), 2 or 3 of 8
 // exponentials by a polynomial on the multiply-add pipes (469, 490), two threads per row (556), the row maximum as a
-// thread's first score (no change: 490 against 487 at the time), output rows stored by four lanes each (no change).
+// thread's first score (no change: 490 against 487 at the time), output rows stored by four lanes each (no change),
+// half tiles of 64 keys with two buffers of scores, so that the next half's scores are there ahead (561: each half pays
+// its waits and the way through tensor memory in full, which costs more than the overlap brings).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -264,6 +264,40 @@ def test_parts_of_a_joint_buffer_and_no_lse(ctx):
     assert torch.equal(p.o, want)
 
 
+def laid_out(x, layout):
+    """A cache with the values of `x` in another layout (with another layout's values where slots share memory)."""
+    pages, page, heads, d = x.shape
+    if layout == "heads outermost":
+        return x.permute(2, 0, 1, 3).contiguous().permute(1, 2, 0, 3)
+    if layout == "slots outermost":
+        return x.transpose(0, 1).contiguous().transpose(0, 1)
+    if layout == "padded":  # no stride a multiple of another
+        strides = (page * (heads * (d + 8) + 16) + 8, heads * (d + 8) + 16, d + 8, 1)
+        y = torch.full((pages * strides[0],), math.nan, dtype=x.dtype, device="cuda").as_strided(x.shape, strides)
+        return y.copy_(x)
+    if layout == "one head for all":
+        return x[:, :, :1].expand(-1, -1, heads, -1)
+    assert layout == "slots overlap"
+    flat = x[:, :, :, 0].nan_to_num(1).flatten().repeat(d)
+    return flat.as_strided(x.shape, (page * 8 + 16, 8, pages * (page * 8 + 16) + 8, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["heads outermost", "slots outermost", "padded", "one head for all", "slots overlap"])
+@pytest.mark.parametrize("dtype,lens", [("bf16", [(70, 500), (1, 90), (300, 300)]), ("f32", [(9, 200), (1, 90)])])
+def test_cache_layouts(ctx, layout, dtype, lens):
+    p = Problem(dtype, 4, 2, 64, 16, lens, seed=14)
+    p.k, p.v = laid_out(p.k, layout), laid_out(p.v, layout)
+    p.run(ctx)
+    ctx.synchronize(stream())
+    p.check()
+    joint = torch.stack([p.k, p.v], dim=1)  # keys and values of a page side by side
+    p.k, p.v = joint[:, 0], joint[:, 1]
+    p.o.fill_(7)
+    p.run(ctx)
+    p.check()  # (not the same bits: the layout may choose the kernel)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens", [[(1, 100), (1, 40)], [(200, 700), (1, 40)]])
 def test_bad_device_data_is_not_accessed_and_reported(ctx, lens):
