@@ -223,6 +223,28 @@ template <int kThreads, typename G> __device__ __forceinline__ Line lay_line(con
   return line;
 }
 
+// Item w of all, in the order of the sequences, their heads and their blocks, found by the block together: its
+// sequence in scratch.b, whose first item is scratch.start. False when there are no more than w.
+template <int kThreads, typename G> __device__ __forceinline__ bool find_item(const PagedParams &P, int w, LineScratch<kThreads> &scratch) {
+  int64_t before = 0;
+  for (int base = 0; base < P.batch; base += kThreads) {
+    const int b = base + static_cast<int>(threadIdx.x);
+    const int64_t mine = b < P.batch ? static_cast<int64_t>(sequence<G>(P, b).blocks) * P.k_heads : 0;
+    int64_t inclusive;
+    const int64_t all = block_scan<kThreads>(mine, inclusive, scratch.warp_sum);
+    if (w < before + all) {
+      if (w >= before + inclusive - mine && w < before + inclusive) {
+        scratch.b = b;
+        scratch.start = before + inclusive - mine;
+      }
+      __syncthreads();
+      return true;
+    }
+    before += all;
+  }
+  return false;
+}
+
 // The item that worker w's stretch begins inside of, if no earlier stretch does (parts 0 otherwise). Its part 0
 // lies in slot 2 (w - 1) + 1, part p in slot 2 (w - 1 + p).
 struct alignas(32) SplitItem {

@@ -218,13 +218,48 @@ __device__ __forceinline__ void value_tile(const float (&p)[2][4], uint32_t tile
   }
 }
 
-template <typename T, int kDim> __device__ __forceinline__ void attention_body(const PagedParams &P) {
+// Blocks of a cluster: barrier (every block makes the same number of arrivals, whatever it finds to do), and the
+// shared memory of block `rank` at this block's address.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t address_in(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 load2_cluster(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 load4_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+constexpr int kMaxCluster = 8;
+
+// kJoint: a cluster takes one item, each of its blocks a part of the keys, and adds the parts up through its shared
+// memory. One launch and no workspace, for few items with keys enough for several blocks (see the host's rule).
+template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void attention_body(const PagedParams &P) {
   using Cfg = Config<T, kDim>;
   using Cut = typename Cfg::Cut;
   constexpr int kThreads = Cfg::kThreads, kWarps = Cfg::kWarps, kUnit = Cfg::kUnit;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ khp::LineScratch<kThreads> scratch;
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+  __shared__ float2 s_ml[kJoint ? kRows : 1]; // of the block
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t ring = smem_addr(smem) + warp * Cfg::kRing;
   if (P.head_dim < kDim) { // columns that no copy writes count as zeros
@@ -233,17 +268,28 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
   }
   khd::grid_dependency_wait();
   khd::grid_dependents_may_launch();
-  const int w = blockIdx.x;
-  const khp::Line line = khp::lay_line<kThreads, Cut>(P, w, scratch);
-  if (w >= line.workers) {
-    if (threadIdx.x == 0 && !P.whole) P.split_items[w] = khp::SplitItem{};
-    return;
+  const int ranks = kJoint ? static_cast<int>(cluster_size()) : 1, rank = kJoint ? static_cast<int>(cluster_rank()) : 0;
+  const int w = static_cast<int>(blockIdx.x) / ranks;
+  khp::Line line{};
+  int64_t from = 0, until = 1;
+  if constexpr (kJoint) {
+    if (!khp::find_item<kThreads, Cut>(P, w, scratch)) {
+      cluster_barrier();
+      cluster_barrier();
+      return;
+    }
+  } else {
+    line = khp::lay_line<kThreads, Cut>(P, w, scratch);
+    if (w >= line.workers) {
+      if (threadIdx.x == 0 && !P.whole) P.split_items[w] = khp::SplitItem{};
+      return;
+    }
+    from = line.stretch(w), until = line.stretch(w + 1);
   }
-  const int64_t from = line.stretch(w), until = line.stretch(w + 1);
   int64_t at = from, start = scratch.start;
   int b = scratch.b;
   khp::Sequence s = khp::sequence<Cut>(P, b);
-  if (P.whole) { // the first item that begins here
+  if (!kJoint && P.whole) { // the first item that begins here
     const khp::Item item = khp::item_at<Cut>(P, s, start, at);
     if (item.begin < at) at = item.end;
   }
@@ -251,19 +297,30 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
   const bool whole_steps = P.page_size % kKeys == 0; // a step's keys lie in one page
   const int chunks_per_row = P.head_dim * static_cast<int>(sizeof(T)) / 16; // 16-byte pieces that exist
   while (at < until) {
-    while (at >= start + s.head_span * P.k_heads) { // on to the next sequence that has rows
-      start += s.head_span * P.k_heads;
-      s = khp::sequence<Cut>(P, ++b);
-    }
-    const khp::Item item = khp::item_at<Cut>(P, s, start, at);
-    if (at - item.begin >= item.keys.units) { // what is left of the item is only what stands for its end
-      if (threadIdx.x == 0 && at == from && !P.whole) P.split_items[w] = khp::SplitItem{};
-      at = item.end;
-      continue;
+    khp::Item item;
+    int unit0, unit1;
+    if constexpr (kJoint) {
+      item.h = static_cast<int>(w - start) / s.blocks;
+      item.block = static_cast<int>(w - start) - item.h * s.blocks;
+      item.keys = khp::keys_of<Cut>(P, s, item.block);
+      item.begin = 0, item.end = 1;
+      unit0 = static_cast<int>(static_cast<int64_t>(item.keys.units) * rank / ranks);
+      unit1 = static_cast<int>(static_cast<int64_t>(item.keys.units) * (rank + 1) / ranks);
+    } else {
+      while (at >= start + s.head_span * P.k_heads) { // on to the next sequence that has rows
+        start += s.head_span * P.k_heads;
+        s = khp::sequence<Cut>(P, ++b);
+      }
+      item = khp::item_at<Cut>(P, s, start, at);
+      if (at - item.begin >= item.keys.units) { // what is left of the item is only what stands for its end
+        if (threadIdx.x == 0 && at == from && !P.whole) P.split_items[w] = khp::SplitItem{};
+        at = item.end;
+        continue;
+      }
+      unit0 = static_cast<int>(at - item.begin);
+      unit1 = P.whole ? item.keys.units : static_cast<int>(min((until < item.end ? until : item.end) - item.begin, static_cast<int64_t>(item.keys.units)));
     }
     const int h = item.h;
-    const int unit0 = static_cast<int>(at - item.begin);
-    const int unit1 = P.whole ? item.keys.units : static_cast<int>(min((until < item.end ? until : item.end) - item.begin, static_cast<int64_t>(item.keys.units)));
     const int row0 = item.block * kRows, rows_here = min(kRows, s.rows - row0);
     const int t_first = row0 / P.group, t_last = (row0 + rows_here - 1) / P.group;
     const int past = s.kv - s.tokens; // position of token 0 (negative: its first tokens see nothing)
@@ -367,7 +424,7 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
     look_up(0);
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i);
-    if (threadIdx.x == 0 && at == from && !P.whole) khp::note_split<Cut>(P, line, w, s, item); // while the first copies fly
+    if (!kJoint && threadIdx.x == 0 && at == from && !P.whole) khp::note_split<Cut>(P, line, w, s, item); // while the first copies fly
     for (int i = 0; i < steps; ++i) {
       __syncwarp(); // every lane is done with the slot that is refilled now
       issue(i + kStages - 1);
@@ -456,7 +513,20 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
         *reinterpret_cast<float2 *>(mine + (g + 8 * i2) * kPitchF + n * 8 + 2 * (lane & 3)) = make_float2(o[n][2 * i2] * f, o[n][2 * i2 + 1] * f);
     }
     __syncthreads();
-    const bool whole = unit0 == 0 && unit1 == item.keys.units;
+    const bool whole = !kJoint && unit0 == 0 && unit1 == item.keys.units;
+    const auto put = [&](int r, int c, float top, float sum, float (&v)[4]) { // the finished values c .. c + 3 of a row
+      const int t = (row0 + r) / P.group, head = h * P.group + (row0 + r) - t * P.group;
+      const float inv = 1.f / sum;
+      if (c < P.head_dim) {
+        T *dst = reinterpret_cast<T *>(P.o) + (s.q0 + t) * P.o_token + head * P.o_head + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = sum != 0.f ? v[j] * inv : 0.f; // a row that sees no key: zeros
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+        else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]));
+      }
+      if (c == 0 && P.lse != nullptr)
+        P.lse[static_cast<int64_t>(s.q0 + t) * (P.k_heads * P.group) + head] = sum != 0.f ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+    };
     const int64_t part = item.begin < from ? 2 * static_cast<int64_t>(w) : 2 * static_cast<int64_t>(w) + 1;
     for (int i = threadIdx.x; i < rows_here * (kDim / 4); i += kThreads) {
       const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
@@ -471,22 +541,45 @@ template <typename T, int kDim> __device__ __forceinline__ void attention_body(c
         const float4 y = *reinterpret_cast<const float4 *>(smem + x * Cfg::kRing + (r * kPitchF + c) * 4);
         v[0] += y.x, v[1] += y.y, v[2] += y.z, v[3] += y.w;
       }
+      if constexpr (kJoint) { // this thread alone has read these places
+        *reinterpret_cast<float4 *>(smem + (r * kPitchF + c) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+        if (c == 0) s_ml[r] = make_float2(top, sum);
+        continue;
+      }
       if (!whole) {
         *reinterpret_cast<float4 *>(P.partial_o + (part * kRows + r) * kDim + c) = make_float4(v[0], v[1], v[2], v[3]);
         if (c == 0) P.partial_ml[part * kRows + r] = make_float2(top, sum);
         continue;
       }
-      const int t = (row0 + r) / P.group, head = h * P.group + (row0 + r) - t * P.group;
-      const float inv = 1.f / sum;
-      if (c < P.head_dim) {
-        T *dst = reinterpret_cast<T *>(P.o) + (s.q0 + t) * P.o_token + head * P.o_head + c;
+      put(r, c, top, sum, v);
+    }
+    if constexpr (kJoint) {
+      cluster_barrier();
+      for (int i = rank * kThreads + threadIdx.x; i < rows_here * (kDim / 4); i += ranks * kThreads) {
+        const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
+        float2 ml[kMaxCluster];
+        float4 y[kMaxCluster];
+        float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = sum != 0.f ? v[j] * inv : 0.f; // a row that sees no key: zeros
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-        else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack<T>(v[0], v[1]), pack<T>(v[2], v[3]));
+        for (int x = 0; x < kMaxCluster; ++x)
+          if (x < ranks) {
+            ml[x] = load2_cluster(address_in(smem_addr(&s_ml[r]), x));
+            y[x] = load4_cluster(address_in(smem_addr(smem) + (r * kPitchF + c) * 4, x));
+            top = fmaxf(top, ml[x].x);
+          }
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < kMaxCluster; ++x)
+          if (x < ranks) {
+            const float f = exp2f(ml[x].x - ref);
+            sum = fmaf(ml[x].y, f, sum);
+            v[0] = fmaf(y[x].x, f, v[0]), v[1] = fmaf(y[x].y, f, v[1]), v[2] = fmaf(y[x].z, f, v[2]), v[3] = fmaf(y[x].w, f, v[3]);
+          }
+        put(r, c, top, sum, v);
       }
-      if (c == 0 && P.lse != nullptr)
-        P.lse[static_cast<int64_t>(s.q0 + t) * (P.k_heads * P.group) + head] = sum != 0.f ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+      cluster_barrier(); // no block leaves while another reads from it
+      return;
     }
     __syncthreads(); // the scratch becomes rings again
     if (P.head_dim < kDim) { // and their unwritten columns zeros
@@ -507,7 +600,9 @@ template <typename T, int kDim> __device__ __forceinline__ void combine(const Pa
 
 #define KH_PAGED(suffix, T, dim)                                                                                              \
   extern "C" __global__ void __launch_bounds__(Config<T, dim>::kThreads)                                                      \
-  paged_attention_##suffix##_##dim(const __grid_constant__ PagedParams P) { attention_body<T, dim>(P); }                      \
+  paged_attention_##suffix##_##dim(const __grid_constant__ PagedParams P) { attention_body<T, dim, false>(P); }               \
+  extern "C" __global__ void __launch_bounds__(Config<T, dim>::kThreads)                                                      \
+  paged_attention_joint_##suffix##_##dim(const __grid_constant__ PagedParams P) { attention_body<T, dim, true>(P); }          \
   extern "C" __global__ void __launch_bounds__(256) paged_attention_combine_##suffix##_##dim(                                 \
       const __grid_constant__ PagedParams P) { combine<T, dim>(P); }
 

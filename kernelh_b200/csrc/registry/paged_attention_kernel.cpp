@@ -15,6 +15,9 @@ constexpr int kRows = 16, kUnit = 64;                  // kernels/paged_attentio
 constexpr int kChunkRows = 256, kChunkKeys = 128;      // kernels/paged_attention_chunk.cu
 constexpr int kMinUnits = 2;          // units per worker below which more workers cost more than they bring
 constexpr int kWholeKeys = 512;       // see run_paged_attention
+constexpr int kMaxCluster = 8;        // kernels/paged_attention.cu
+// Keys per block of a cluster up to which it is used, see run_paged_attention.
+constexpr int64_t joint_keys(int32_t dtype) { return dtype == KH_F32 ? 256 : 384; }
 constexpr long kMaxSms = 160;         // workspaces are sized for at most this many SMs
 
 int element_size(int32_t dtype) { return dtype == KH_F32 ? 4 : 2; }
@@ -178,13 +181,14 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
   p.scale_log2 = a.scale * 1.4426950408889634f;
   const std::string suffix = std::string(a.dtype == KH_F32 ? "f32_" : a.dtype == KH_BF16 ? "bf16_" : "f16_") + std::to_string(s.dim);
   const auto launch = [&](const char *image, const std::string &entry, LaunchDims grid, unsigned threads, size_t smem,
-                          std::initializer_list<TensorMapBytes> maps, int box_rows) -> Result<void> {
+                          std::initializer_list<TensorMapBytes> maps, int box_rows, unsigned cluster = 1) -> Result<void> {
     LaunchStep step;
     step.entry = entry;
     step.grid = grid;
     step.block = {threads, 1, 1};
     step.dynamic_smem = smem;
     step.overlap_tail = true;
+    step.cluster = cluster;
     LaunchArgs args;
     args.add_struct_bytes(&p, sizeof p);
     for (const TensorMapBytes &m : maps) args.add_tensor_map(m);
@@ -252,6 +256,17 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
     if (alone) return {};
     p.rows_above = 0, p.rows_upto = kRows;
   }
+  // Few items: each to a cluster of as many blocks as fit on the device at once and have keys to work on; one launch. Up to
+  // the point where more blocks than a cluster has bring in the keys faster. (Replayed from a graph, 32 heads over 8 of 128 in
+  // bf16, against a stretch of the line per block: one sequence of 400 keys 10.3 us against 12.4, 8 of
+  // 1000 16.5 against 18.5, one of 4000 14.5 both, two of 4000 18.5 against 16.5. fp32, 8 x 1000 with 16 heads of 64, two blocks each 24.7 against
+  // 20.7, but one of 1000 12.4 against 14.5: its arithmetic takes three times as long.)
+  const int64_t few = item_count(a, kRows), units = (static_cast<int64_t>(a.max_kv_len) + kUnit - 1) / kUnit;
+  int64_t ranks = kMaxCluster;
+  while (ranks > 1 && (few * ranks > s.per_sm * sms || ranks > units)) ranks /= 2;
+  if (ranks > 1 && a.max_kv_len <= ranks * joint_keys(a.dtype))
+    return launch("paged_attention", "paged_attention_joint_" + suffix, {static_cast<unsigned>(few * ranks), 1, 1}, 32u * s.warps, s.smem, {}, 0,
+                  static_cast<unsigned>(ranks));
   // Short key ranges are not split: an item takes less than the second launch that would add its parts up. (Replayed
   // from a graph, 32 heads over 8 of 128 in bf16: 8 sequences of 200 keys 10.4 us against 13.4, 64 of 400 keys 27.1
   // against 34.7, one of 800 keys 16.6 against 12.4, 64 of 800 keys 45.6 against 51.8.)

@@ -181,6 +181,13 @@ CASES = [  # dtype, q heads, k heads, head_dim, page, lengths, heads first, opti
     ("bf16", 8, 2, 128, 16, CHUNKS, False, dict(causal=False)), ("f16", 4, 2, 64, 16, CHUNKS, False, dict(causal=False, window=70)),
     ("bf16", 8, 2, 128, 16, CHUNKS, False, dict(window=1)), ("f16", 8, 1, 96, 32, CHUNKS, False, dict(window=100)),
     ("f32", 2, 2, 64, 16, CHUNKS, False, dict(window=17)), ("bf16", 8, 1, 64, 16, EDGES, False, dict(window=40)),
+    # the same lengths with a long one among them
+    ("bf16", 8, 2, 128, 16, EDGES + [(1, 9001)], False, {}), ("f32", 4, 4, 64, 64, EDGES + [(1, 9001)], False, {}), ("f16", 4, 4, 64, 8, EDGES + [(2, 5000)], True, {}),
+    ("bf16", 2, 1, 256, 32, EDGES + [(1, 9001)], False, {}), ("f32", 3, 1, 256, 5, EDGES + [(3, 2500)], False, dict(window=700)), ("bf16", 5, 1, 80, 1, EDGES + [(1, 4500)], False, {}),
+    ("bf16", 2, 1, 256, 16, CHUNKS + [(7, 6000)], False, dict(window=3000)), ("f32", 4, 2, 128, 16, CHUNKS + [(7, 2200)], False, {}),
+    # one item for every two, four or eight blocks of a cluster; rows that see nothing; one key
+    ("bf16", 16, 16, 64, 16, [(1, 70 + b) for b in range(8)], False, {}), ("f16", 8, 8, 128, 32, [(1, 300), (1, 1), (2, 900)], False, dict(window=64)),
+    ("f32", 8, 4, 128, 16, [(4, 2), (2, 500)], False, {}), ("bf16", 8, 2, 256, 8, [(1, 2000)], True, dict(causal=False)),
     # more new tokens than keys: the first queries see nothing
     ("bf16", 4, 2, 128, 16, [(9, 4), (70, 3), (3, 0)], False, {}), ("f32", 4, 2, 64, 16, [(9, 4), (40, 20)], False, dict(causal=False)),
     # one long sequence over all workers; many short ones
@@ -243,8 +250,10 @@ def test_a_nan_stays_with_those_who_see_it(ctx, dtype, d, n):
 def test_lengths_beyond_the_hints(ctx):
     for dtype in ("bf16", "f32"):
         p = Problem(dtype, 8, 2, 128, 16, [(300, 900), (1, 1500)], seed=6)
-        p.run(ctx, hints=dict(max_q_len=1, max_kv_len=1))
-        p.check()
+        for keys in (1, 200, 5000):
+            p.o[:p.tokens] = math.nan
+            p.run(ctx, hints=dict(max_q_len=1, max_kv_len=keys))
+            p.check()
 
 
 @pytest.mark.gpu
@@ -347,7 +356,7 @@ def test_no_tokens_and_no_sequences(ctx):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,grown", [("bf16", [(1, 901), (1, 3), (1, 77)]), ("f32", [(1, 901), (1, 3), (1, 77)]),
-                                         ("bf16", [(1, 30), (200, 900), (61, 400)])])
+                                         ("bf16", [(1, 30), (200, 900), (61, 400)]), ("bf16", [(1, 9001), (1, 3), (2, 4000)])])
 def test_a_captured_call_follows_the_lengths(ctx, dtype, grown):
     """Captured with one set of lengths, replayed with others; two graphs at once on two streams, each with its
     own workspace."""
