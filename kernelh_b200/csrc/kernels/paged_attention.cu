@@ -9,6 +9,7 @@
 // warps are added up at the end of the item, through shared memory, in a fixed order.
 //   S = Q K^T and O += P V run as mma.sync m16n8k16 (16-bit types) or as three m16n8k8 tf32 products of
 //   hi/lo parts of 11 significant bits each (fp32; lo.lo is dropped: 2^-22 of a product).
+// A single fp32 row takes plain multiply-adds (score_row). Few items go to clusters, an item to each (kJoint).
 // HBM-bound at decoding: 4 rows x 128 values of queries cost 0.5 flop per byte of cache per row, far below
 // what any matrix unit needs; what counts is bytes in flight: two 16-key stages of keys and values per
 // warp, 8 warps per SM, are 128 KiB. Scores, softmax and sums are fp32; P is rounded to the values' type for
@@ -218,6 +219,50 @@ __device__ __forceinline__ void value_tile(const float (&p)[2][4], uint32_t tile
   }
 }
 
+// A single row in fp32: 15 of 16 rows of the products above would be padding, at seven instructions for every value that
+// is split. Plain multiply-adds instead: scores with two lanes to a key, each half of its values, handed out in the
+// layout above with the row in the place of all eight; P V with the lanes along head_dim, lane i's values 64 x + 2 i (+1) in
+// o[2 x][0] and o[2 x + 1][0]. (8 sequences of up to 1024 keys, 16 heads of 64: 16.5 us from a graph
+// against 20.6; one of 1000 keys 10.4 against 12.4.)
+template <int kDim> __device__ __forceinline__ void score_row(uint32_t q, uint32_t tile, float (&s)[2][4]) {
+  constexpr int kPitch = Config<float, kDim>::kPitch;
+  const int lane = threadIdx.x & 31;
+  const uint32_t k = tile + (lane & 15) * kPitch + (lane >> 4) * (kDim * 2);
+  q += (lane >> 4) * (kDim * 2);
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < kDim / 8; ++i) {
+    float4 a, b;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w) : "r"(q + i * 16) : "memory");
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w) : "r"(k + i * 16) : "memory");
+    sum[0] = __ffma2_rn(make_float2(a.x, a.y), make_float2(b.x, b.y), sum[0]);
+    sum[1] = __ffma2_rn(make_float2(a.z, a.w), make_float2(b.z, b.w), sum[1]);
+  }
+  float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+  all += __shfl_xor_sync(0xffffffffu, all, 16);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[t][j] = __shfl_sync(0xffffffffu, all, 8 * t + 2 * (lane & 3) + j);
+    s[t][2] = s[t][3] = 0.f;
+  }
+}
+template <int kDim> __device__ __forceinline__ void value_row(const float (&p)[2][4], uint32_t tile, float (&o)[kDim / 8][4]) {
+  constexpr int kPitch = Config<float, kDim>::kPitch;
+  const uint32_t at = tile + (threadIdx.x & 31) * 8;
+#pragma unroll
+  for (int k = 0; k < kKeys; ++k) {
+    const float w = __shfl_sync(0xffffffffu, p[k >> 3][k & 1], (k & 7) >> 1);
+#pragma unroll
+    for (int x = 0; x < kDim / 64; ++x) {
+      float2 v;
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at + k * kPitch + x * 256) : "memory");
+      o[2 * x][0] = fmaf(w, v.x, o[2 * x][0]);
+      o[2 * x + 1][0] = fmaf(w, v.y, o[2 * x + 1][0]);
+    }
+  }
+}
+
 // Blocks of a cluster: barrier (every block makes the same number of arrivals, whatever it finds to do), and the
 // shared memory of block `rank` at this block's address.
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -331,6 +376,7 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
 
     // this lane's two rows: their queries and the keys they see
     const int g = lane >> 2;
+    const bool one = sizeof(T) == 4 && rows_here == 1; // see score_row: every lane's first row is the one
     int see_lo[2], see_hi[2];
     const T *q_row[2];
 #pragma unroll
@@ -339,8 +385,9 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
       const bool real = r < s.rows;
       const int t = real ? r / P.group : 0, head = h * P.group + (real ? r - t * P.group : 0);
       q_row[i] = real ? reinterpret_cast<const T *>(P.q) + (s.q0 + t) * P.q_token + head * P.q_head : nullptr;
-      see_hi[i] = !real ? -1 : P.causal ? past + t : s.kv - 1;
-      const int64_t first = P.window > 0 ? static_cast<int64_t>(past) + t - P.window + 1 : 0;
+      const int t_seen = one ? t_first : t;
+      see_hi[i] = !real && !(one && i == 0) ? -1 : P.causal ? past + t_seen : s.kv - 1;
+      const int64_t first = P.window > 0 ? static_cast<int64_t>(past) + t_seen - P.window + 1 : 0;
       see_lo[i] = static_cast<int>(first > 0 ? first : 0);
     }
     // what all real rows of the warp's tile see: a step inside needs no mask (rows that are not real are not stored)
@@ -434,7 +481,12 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
       if (key0 >= key_b) continue;
       const uint32_t k_tile = ring + (i % kStages) * 2 * Cfg::kTile;
       float sc[2][4];
-      score_tile<T, kDim>(q, k_tile, sc);
+      if constexpr (sizeof(T) == 4) {
+        if (one) score_row<kDim>(smem_addr(smem) + kWarps * Cfg::kRing, k_tile, sc);
+        else score_tile<T, kDim>(q, k_tile, sc);
+      } else {
+        score_tile<T, kDim>(q, k_tile, sc);
+      }
       float top[2] = {-INFINITY, -INFINITY};
       if (key0 + kKeys - 1 <= all_hi && key0 >= all_lo) {
 #pragma unroll
@@ -485,7 +537,12 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
           sc[t][j] = khd::exp2_approx(sc[t][j] - ref[j >> 1]);
           l[j >> 1] += sc[t][j];
         }
-      value_tile<T, kDim>(sc, k_tile + Cfg::kTile, o);
+      if constexpr (sizeof(T) == 4) {
+        if (one) value_row<kDim>(sc, k_tile + Cfg::kTile, o);
+        else value_tile<T, kDim>(sc, k_tile + Cfg::kTile, o);
+      } else {
+        value_tile<T, kDim>(sc, k_tile + Cfg::kTile, o);
+      }
     }
 
     // the warps' rows are added up: the rings are drained and serve as scratch
@@ -508,6 +565,12 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
 #pragma unroll
       for (int x = 1; x < kWarps; ++x) top = fmaxf(top, s_m[x][g + 8 * i2]);
       const float f = exp2f(m[i2] - (top == -INFINITY ? 0.f : top));
+      if (one) {
+        if (i2 == 0)
+#pragma unroll
+          for (int x = 0; x < kDim / 64; ++x) *reinterpret_cast<float2 *>(mine + 64 * x + 2 * lane) = make_float2(o[2 * x][0] * f, o[2 * x + 1][0] * f);
+        continue;
+      }
 #pragma unroll
       for (int n = 0; n < kDim / 8; ++n)
         *reinterpret_cast<float2 *>(mine + (g + 8 * i2) * kPitchF + n * 8 + 2 * (lane & 3)) = make_float2(o[n][2 * i2] * f, o[n][2 * i2 + 1] * f);

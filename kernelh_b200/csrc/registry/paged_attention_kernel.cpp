@@ -16,8 +16,6 @@ constexpr int kChunkRows = 256, kChunkKeys = 128;      // kernels/paged_attentio
 constexpr int kMinUnits = 2;          // units per worker below which more workers cost more than they bring
 constexpr int kWholeKeys = 512;       // see run_paged_attention
 constexpr int kMaxCluster = 8;        // kernels/paged_attention.cu
-// Keys per block of a cluster up to which it is used, see run_paged_attention.
-constexpr int64_t joint_keys(int32_t dtype) { return dtype == KH_F32 ? 256 : 384; }
 constexpr long kMaxSms = 160;         // workspaces are sized for at most this many SMs
 
 int element_size(int32_t dtype) { return dtype == KH_F32 ? 4 : 2; }
@@ -257,14 +255,17 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
     p.rows_above = 0, p.rows_upto = kRows;
   }
   // Few items: each to a cluster of as many blocks as fit on the device at once and have keys to work on; one launch. Up to
-  // the point where more blocks than a cluster has bring in the keys faster. (Replayed from a graph, 32 heads over 8 of 128 in
-  // bf16, against a stretch of the line per block: one sequence of 400 keys 10.3 us against 12.4, 8 of
-  // 1000 16.5 against 18.5, one of 4000 14.5 both, two of 4000 18.5 against 16.5. fp32, 8 x 1000 with 16 heads of 64, two blocks each 24.7 against
-  // 20.7, but one of 1000 12.4 against 14.5: its arithmetic takes three times as long.)
-  const int64_t few = item_count(a, kRows), units = (static_cast<int64_t>(a.max_kv_len) + kUnit - 1) / kUnit;
+  // the point where more blocks than a cluster has bring in the keys faster: 512 keys a block when the clusters fill more
+  // than half the device, else 384, and 256 for the split products of several fp32 rows. (Replayed from a graph, against a
+  // stretch of the line per block; 32 heads over 8 of 128 in bf16: one sequence of 400 keys 10.3 us against 12.4, 8 of 2000
+  // 20.9 against 22.7, one of 4000 14.5 both, two of 4000 18.5 against 16.5; fp32, 16 heads of 64: 8 of 1000 18.6 against
+  // 20.6, one of 4000 18.0 against 14.8; by split products 8 of 1000 24.7 against 20.7.)
+  const int64_t few = item_count(a, kRows), units = (static_cast<int64_t>(a.max_kv_len) + kUnit - 1) / kUnit, blocks = s.per_sm * sms;
   int64_t ranks = kMaxCluster;
-  while (ranks > 1 && (few * ranks > s.per_sm * sms || ranks > units)) ranks /= 2;
-  if (ranks > 1 && a.max_kv_len <= ranks * joint_keys(a.dtype))
+  while (ranks > 1 && (few * ranks > blocks || ranks > units)) ranks /= 2;
+  const bool several = static_cast<int64_t>(a.max_q_len) * p.group > 1;
+  const int64_t keys = a.dtype == KH_F32 && several ? 256 : 2 * few * ranks > blocks ? 512 : 384; // a block's
+  if (ranks > 1 && a.max_kv_len <= ranks * keys)
     return launch("paged_attention", "paged_attention_joint_" + suffix, {static_cast<unsigned>(few * ranks), 1, 1}, 32u * s.warps, s.smem, {}, 0,
                   static_cast<unsigned>(ranks));
   // Short key ranges are not split: an item takes less than the second launch that would add its parts up. (Replayed
