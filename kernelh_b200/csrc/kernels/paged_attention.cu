@@ -9,7 +9,7 @@
 // warps are added up at the end of the item, through shared memory, in a fixed order.
 //   S = Q K^T and O += P V run as mma.sync m16n8k16 (16-bit types) or as three m16n8k8 tf32 products of
 //   hi/lo parts of 11 significant bits each (fp32; lo.lo is dropped: 2^-22 of a product).
-// A single fp32 row takes plain multiply-adds (score_row). Few items go to clusters, an item to each (kJoint).
+// Up to four fp32 rows take plain multiply-adds (score_rows). Few items go to clusters, an item to each (kJoint).
 // HBM-bound at decoding: 4 rows x 128 values of queries cost 0.5 flop per byte of cache per row, far below
 // what any matrix unit needs; what counts is bytes in flight: two 16-key stages of keys and values per
 // warp, 8 warps per SM, are 128 KiB. Scores, softmax and sums are fp32; P is rounded to the values' type for
@@ -219,46 +219,67 @@ __device__ __forceinline__ void value_tile(const float (&p)[2][4], uint32_t tile
   }
 }
 
-// A single row in fp32: 15 of 16 rows of the products above would be padding, at seven instructions for every value that
-// is split. Plain multiply-adds instead: scores with two lanes to a key, each half of its values, handed out in the
-// layout above with the row in the place of all eight; P V with the lanes along head_dim, lane i's values 64 x + 2 i (+1) in
-// o[2 x][0] and o[2 x + 1][0]. (8 sequences of up to 1024 keys, 16 heads of 64: 16.5 us from a graph
-// against 20.6; one of 1000 keys 10.4 against 12.4.)
-template <int kDim> __device__ __forceinline__ void score_row(uint32_t q, uint32_t tile, float (&s)[2][4]) {
+// Up to kFewRows rows in fp32: most of the 16 rows of the products above would be padding, at seven instructions for every
+// value that is split. Plain multiply-adds instead: scores with two lanes to a key, each half of its values, handed out in
+// the layout above; P V with the lanes along head_dim, lane i's values 64 x + 2 i (+1) of row r in o[(r * kDim / 64 + x)][0 and
+// 1]. kFew of them are worked on, 1 or kFewRows. (8 sequences of up to 1024 keys, 16 heads of 64: 16.5 us from a graph against
+// 20.6; MEASURE.)
+constexpr int kFewRows = 4;
+template <int kDim, int kFew> __device__ __forceinline__ void score_rows(uint32_t q, uint32_t tile, float (&s)[2][4]) {
   constexpr int kPitch = Config<float, kDim>::kPitch;
   const int lane = threadIdx.x & 31;
   const uint32_t k = tile + (lane & 15) * kPitch + (lane >> 4) * (kDim * 2);
   q += (lane >> 4) * (kDim * 2);
-  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  float2 sum[kFew][2];
+#pragma unroll
+  for (int r = 0; r < kFew; ++r) sum[r][0] = sum[r][1] = make_float2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < kDim / 8; ++i) {
-    float4 a, b;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w) : "r"(q + i * 16) : "memory");
+    float4 b;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w) : "r"(k + i * 16) : "memory");
-    sum[0] = __ffma2_rn(make_float2(a.x, a.y), make_float2(b.x, b.y), sum[0]);
-    sum[1] = __ffma2_rn(make_float2(a.z, a.w), make_float2(b.z, b.w), sum[1]);
+#pragma unroll
+    for (int r = 0; r < kFew; ++r) {
+      float4 a;
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w) : "r"(q + r * kPitch + i * 16) : "memory");
+      sum[r][0] = __ffma2_rn(make_float2(a.x, a.y), make_float2(b.x, b.y), sum[r][0]);
+      sum[r][1] = __ffma2_rn(make_float2(a.z, a.w), make_float2(b.z, b.w), sum[r][1]);
+    }
   }
-  float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-  all += __shfl_xor_sync(0xffffffffu, all, 16);
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) s[t][j] = __shfl_sync(0xffffffffu, all, 8 * t + 2 * (lane & 3) + j);
-    s[t][2] = s[t][3] = 0.f;
+    for (int j = 0; j < 4; ++j) s[t][j] = 0.f;
+#pragma unroll
+  for (int r = 0; r < kFew; ++r) {
+    float all = (sum[r][0].x + sum[r][0].y) + (sum[r][1].x + sum[r][1].y);
+    all += __shfl_xor_sync(0xffffffffu, all, 16);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float v = __shfl_sync(0xffffffffu, all, 8 * t + 2 * (lane & 3) + j);
+        if (lane >> 2 == r) s[t][j] = v;
+      }
   }
 }
-template <int kDim> __device__ __forceinline__ void value_row(const float (&p)[2][4], uint32_t tile, float (&o)[kDim / 8][4]) {
+template <int kDim, int kFew> __device__ __forceinline__ void value_rows(const float (&p)[2][4], uint32_t tile, float (&o)[kDim / 8][4]) {
   constexpr int kPitch = Config<float, kDim>::kPitch;
   const uint32_t at = tile + (threadIdx.x & 31) * 8;
 #pragma unroll
   for (int k = 0; k < kKeys; ++k) {
-    const float w = __shfl_sync(0xffffffffu, p[k >> 3][k & 1], (k & 7) >> 1);
+    float w[kFew];
+#pragma unroll
+    for (int r = 0; r < kFew; ++r) w[r] = __shfl_sync(0xffffffffu, p[k >> 3][k & 1], 4 * r + ((k & 7) >> 1));
 #pragma unroll
     for (int x = 0; x < kDim / 64; ++x) {
       float2 v;
       asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at + k * kPitch + x * 256) : "memory");
-      o[2 * x][0] = fmaf(w, v.x, o[2 * x][0]);
-      o[2 * x + 1][0] = fmaf(w, v.y, o[2 * x + 1][0]);
+#pragma unroll
+      for (int r = 0; r < kFew; ++r) {
+        float(&to)[4] = o[r * (kDim / 64) + x];
+        to[0] = fmaf(w[r], v.x, to[0]);
+        to[1] = fmaf(w[r], v.y, to[1]);
+      }
     }
   }
 }
@@ -376,7 +397,7 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
 
     // this lane's two rows: their queries and the keys they see
     const int g = lane >> 2;
-    const bool one = sizeof(T) == 4 && rows_here == 1; // see score_row: every lane's first row is the one
+    const int few = sizeof(T) == 4 && rows_here <= kFewRows ? rows_here : 0; // rows that score_rows takes
     int see_lo[2], see_hi[2];
     const T *q_row[2];
 #pragma unroll
@@ -385,9 +406,8 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
       const bool real = r < s.rows;
       const int t = real ? r / P.group : 0, head = h * P.group + (real ? r - t * P.group : 0);
       q_row[i] = real ? reinterpret_cast<const T *>(P.q) + (s.q0 + t) * P.q_token + head * P.q_head : nullptr;
-      const int t_seen = one ? t_first : t;
-      see_hi[i] = !real && !(one && i == 0) ? -1 : P.causal ? past + t_seen : s.kv - 1;
-      const int64_t first = P.window > 0 ? static_cast<int64_t>(past) + t_seen - P.window + 1 : 0;
+      see_hi[i] = !real ? -1 : P.causal ? past + t : s.kv - 1;
+      const int64_t first = P.window > 0 ? static_cast<int64_t>(past) + t - P.window + 1 : 0;
       see_lo[i] = static_cast<int>(first > 0 ? first : 0);
     }
     // what all real rows of the warp's tile see: a step inside needs no mask (rows that are not real are not stored)
@@ -482,7 +502,8 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
       const uint32_t k_tile = ring + (i % kStages) * 2 * Cfg::kTile;
       float sc[2][4];
       if constexpr (sizeof(T) == 4) {
-        if (one) score_row<kDim>(smem_addr(smem) + kWarps * Cfg::kRing, k_tile, sc);
+        if (few == 1) score_rows<kDim, 1>(smem_addr(smem) + kWarps * Cfg::kRing, k_tile, sc);
+        else if (few > 0) score_rows<kDim, kFewRows>(smem_addr(smem) + kWarps * Cfg::kRing, k_tile, sc);
         else score_tile<T, kDim>(q, k_tile, sc);
       } else {
         score_tile<T, kDim>(q, k_tile, sc);
@@ -521,6 +542,19 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
           const float f = khd::exp2_approx(m[i2] - (m_new == -INFINITY ? 0.f : m_new));
           m[i2] = m_new;
           l[i2] *= f;
+          if (few > 0) { // o is laid out along head_dim
+            if (i2 == 0)
+#pragma unroll
+              for (int r = 0; r < kFewRows; ++r) {
+                const float f_row = __shfl_sync(0xffffffffu, f, 4 * r);
+#pragma unroll
+                for (int x = 0; x < kDim / 64; ++x) {
+                  o[r * (kDim / 64) + x][0] *= f_row;
+                  o[r * (kDim / 64) + x][1] *= f_row;
+                }
+              }
+            continue;
+          }
 #pragma unroll
           for (int n = 0; n < kDim / 8; ++n) {
             o[n][2 * i2] *= f;
@@ -538,7 +572,8 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
           l[j >> 1] += sc[t][j];
         }
       if constexpr (sizeof(T) == 4) {
-        if (one) value_row<kDim>(sc, k_tile + Cfg::kTile, o);
+        if (few == 1) value_rows<kDim, 1>(sc, k_tile + Cfg::kTile, o);
+        else if (few > 0) value_rows<kDim, kFewRows>(sc, k_tile + Cfg::kTile, o);
         else value_tile<T, kDim>(sc, k_tile + Cfg::kTile, o);
       } else {
         value_tile<T, kDim>(sc, k_tile + Cfg::kTile, o);
@@ -565,10 +600,18 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
 #pragma unroll
       for (int x = 1; x < kWarps; ++x) top = fmaxf(top, s_m[x][g + 8 * i2]);
       const float f = exp2f(m[i2] - (top == -INFINITY ? 0.f : top));
-      if (one) {
+      if (few > 0) {
         if (i2 == 0)
 #pragma unroll
-          for (int x = 0; x < kDim / 64; ++x) *reinterpret_cast<float2 *>(mine + 64 * x + 2 * lane) = make_float2(o[2 * x][0] * f, o[2 * x + 1][0] * f);
+          for (int r = 0; r < kFewRows; ++r) {
+            const float f_row = __shfl_sync(0xffffffffu, f, 4 * r);
+            if (r < few)
+#pragma unroll
+              for (int x = 0; x < kDim / 64; ++x) {
+                const float(&from_row)[4] = o[r * (kDim / 64) + x];
+                *reinterpret_cast<float2 *>(mine + r * kPitchF + 64 * x + 2 * lane) = make_float2(from_row[0] * f_row, from_row[1] * f_row);
+              }
+          }
         continue;
       }
 #pragma unroll
