@@ -9,7 +9,7 @@
 // warps are added up at the end of the item, through shared memory, in a fixed order.
 //   S = Q K^T and O += P V run as mma.sync m16n8k16 (16-bit types) or as three m16n8k8 tf32 products of
 //   hi/lo parts of 11 significant bits each (fp32; lo.lo is dropped: 2^-22 of a product).
-// Up to four fp32 rows take plain multiply-adds (score_rows). Few items go to clusters, an item to each (kJoint).
+// Few fp32 rows take plain multiply-adds (score_rows). Few items go to clusters, an item to each (kJoint).
 // HBM-bound at decoding: 4 rows x 128 values of queries cost 0.5 flop per byte of cache per row, far below
 // what any matrix unit needs; what counts is bytes in flight: two 16-key stages of keys and values per
 // warp, 8 warps per SM, are 128 KiB. Scores, softmax and sums are fp32; P is rounded to the values' type for
@@ -219,12 +219,14 @@ __device__ __forceinline__ void value_tile(const float (&p)[2][4], uint32_t tile
   }
 }
 
-// Up to kFewRows rows in fp32: most of the 16 rows of the products above would be padding, at seven instructions for every
-// value that is split. Plain multiply-adds instead: scores with two lanes to a key, each half of its values, handed out in
-// the layout above; P V with the lanes along head_dim, lane i's values 64 x + 2 i (+1) of row r in o[(r * kDim / 64 + x)][0 and
-// 1]. kFew of them are worked on, 1 or kFewRows. (8 sequences of up to 1024 keys, 16 heads of 64: 16.5 us from a graph against
-// 20.6; MEASURE.)
-constexpr int kFewRows = 4;
+// Few rows in fp32: most of the 16 rows of the products above would be padding, at seven instructions for every value that
+// is split. Plain multiply-adds instead: scores with two lanes to a key, each half of its values, handed out in the
+// layout above; P V with the lanes along head_dim, lane i's values 64 x + 2 i (+1) of row r in o[r * kDim / 64 + x][0 and 1].
+// kFew rows are worked on: 1, 4, or 8 for longer rows than 64. (From a graph, against split products: 8 sequences of up to
+// 1024 keys, 16 heads of 64, one row each, 16.5 us against 20.6. 16 x 8192 keys, 8 key/value heads: 4 rows of 64 values 122 against
+// 149, of 128 214 against 430, 3 of 256 647 against 1669; 8 rows of 128 345 against 461, of 256 1399 against 1693, but 6 of
+// 64 176 against 157.)
+template <int kDim> constexpr int kFewRows = kDim == 64 ? 4 : 8;
 template <int kDim, int kFew> __device__ __forceinline__ void score_rows(uint32_t q, uint32_t tile, float (&s)[2][4]) {
   constexpr int kPitch = Config<float, kDim>::kPitch;
   const int lane = threadIdx.x & 31;
@@ -397,7 +399,7 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
 
     // this lane's two rows: their queries and the keys they see
     const int g = lane >> 2;
-    const int few = sizeof(T) == 4 && rows_here <= kFewRows ? rows_here : 0; // rows that score_rows takes
+    const int few = sizeof(T) == 4 && rows_here <= kFewRows<kDim> ? rows_here : 0; // rows that score_rows takes
     int see_lo[2], see_hi[2];
     const T *q_row[2];
 #pragma unroll
@@ -503,7 +505,8 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
       float sc[2][4];
       if constexpr (sizeof(T) == 4) {
         if (few == 1) score_rows<kDim, 1>(smem_addr(smem) + kWarps * Cfg::kRing, k_tile, sc);
-        else if (few > 0) score_rows<kDim, kFewRows>(smem_addr(smem) + kWarps * Cfg::kRing, k_tile, sc);
+        else if (few > 0 && few <= 4) score_rows<kDim, 4>(smem_addr(smem) + kWarps * Cfg::kRing, k_tile, sc);
+        else if (kFewRows<kDim> > 4 && few > 0) score_rows<kDim, kFewRows<kDim>>(smem_addr(smem) + kWarps * Cfg::kRing, k_tile, sc);
         else score_tile<T, kDim>(q, k_tile, sc);
       } else {
         score_tile<T, kDim>(q, k_tile, sc);
@@ -545,7 +548,7 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
           if (few > 0) { // o is laid out along head_dim
             if (i2 == 0)
 #pragma unroll
-              for (int r = 0; r < kFewRows; ++r) {
+              for (int r = 0; r < kFewRows<kDim>; ++r) {
                 const float f_row = __shfl_sync(0xffffffffu, f, 4 * r);
 #pragma unroll
                 for (int x = 0; x < kDim / 64; ++x) {
@@ -573,7 +576,8 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
         }
       if constexpr (sizeof(T) == 4) {
         if (few == 1) value_rows<kDim, 1>(sc, k_tile + Cfg::kTile, o);
-        else if (few > 0) value_rows<kDim, kFewRows>(sc, k_tile + Cfg::kTile, o);
+        else if (few > 0 && few <= 4) value_rows<kDim, 4>(sc, k_tile + Cfg::kTile, o);
+        else if (kFewRows<kDim> > 4 && few > 0) value_rows<kDim, kFewRows<kDim>>(sc, k_tile + Cfg::kTile, o);
         else value_tile<T, kDim>(sc, k_tile + Cfg::kTile, o);
       } else {
         value_tile<T, kDim>(sc, k_tile + Cfg::kTile, o);
@@ -603,7 +607,7 @@ template <typename T, int kDim, bool kJoint> __device__ __forceinline__ void att
       if (few > 0) {
         if (i2 == 0)
 #pragma unroll
-          for (int r = 0; r < kFewRows; ++r) {
+          for (int r = 0; r < kFewRows<kDim>; ++r) {
             const float f_row = __shfl_sync(0xffffffffu, f, 4 * r);
             if (r < few)
 #pragma unroll

@@ -256,10 +256,10 @@ Result<void> run_paged_attention(Executor &ex, kh_paged_attention_args a, Stream
   }
   // Few items: each to a cluster of as many blocks as fit on the device at once and have keys to work on; one launch. Up to
   // the point where more blocks than a cluster has bring in the keys faster: 512 keys a block when the clusters fill more
-  // than half the device, else 384, and 256 for the split products of several fp32 rows. (Replayed from a graph, against a
+  // than half the device, else 384, and 256 for several fp32 rows, whose arithmetic counts. (Replayed from a graph, against a
   // stretch of the line per block; 32 heads over 8 of 128 in bf16: one sequence of 400 keys 10.3 us against 12.4, 8 of 2000
   // 20.9 against 22.7, one of 4000 14.5 both, two of 4000 18.5 against 16.5; fp32, 16 heads of 64: 8 of 1000 18.6 against
-  // 20.6, one of 4000 18.0 against 14.8; by split products 8 of 1000 24.7 against 20.7.)
+  // 20.6, one of 4000 18.0 against 14.8; by split products, the slowest, 8 of 1000 24.7 against 20.7.)
   const int64_t few = item_count(a, kRows), units = (static_cast<int64_t>(a.max_kv_len) + kUnit - 1) / kUnit, blocks = s.per_sm * sms;
   int64_t ranks = kMaxCluster;
   while (ranks > 1 && (few * ranks > blocks || ranks > units)) ranks /= 2;

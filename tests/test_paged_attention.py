@@ -190,7 +190,8 @@ CASES = [  # dtype, q heads, k heads, head_dim, page, lengths, heads first, opti
     ("f32", 8, 4, 128, 16, [(4, 2), (2, 500)], False, {}), ("bf16", 8, 2, 256, 8, [(1, 2000)], True, dict(causal=False)),
     # one row of fp32, split over blocks, over a cluster and whole
     ("f32", 2, 2, 256, 5, EDGES, False, {}), ("f32", 3, 3, 80, 16, EDGES + [(1, 9001)], True, dict(window=40)), ("f32", 2, 2, 128, 64, EDGES, False, dict(causal=False)),
-    ("f32", 5, 5, 128, 24, [(1, 700)] * 3 + [(1, 0)], False, dict(scale=-0.2)), ("f32", 1, 1, 8, 16, [(1, 40), (3, 90)], False, {}), ("f32", 16, 16, 64, 16, [(1, 1 + 7 * b) for b in range(64)], False, {}),
+    ("f32", 5, 5, 128, 24, [(1, 700)] * 3 + [(1, 0)], False, dict(scale=-0.2)), ("f32", 1, 1, 8, 16, [(1, 40), (3, 90)], False, {}),
+    ("f32", 8, 1, 256, 16, EDGES + [(1, 5000)], False, {}), ("f32", 12, 2, 64, 8, EDGES, True, {}), ("f32", 10, 2, 112, 16, EDGES + [(1, 5000)], False, dict(window=500)), ("f32", 4, 2, 200, 16, [(1, 900), (2, 60), (4, 33)], False, {}), ("f32", 16, 16, 64, 16, [(1, 1 + 7 * b) for b in range(64)], False, {}),
     # more new tokens than keys: the first queries see nothing
     ("bf16", 4, 2, 128, 16, [(9, 4), (70, 3), (3, 0)], False, {}), ("f32", 4, 2, 64, 16, [(9, 4), (40, 20)], False, dict(causal=False)),
     # one long sequence over all workers; many short ones
